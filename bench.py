@@ -224,10 +224,8 @@ def main():
     use_dist = world > 1 or os.environ.get("VITA_BENCH_FORCE_DIST") == "1"
     if use_dist:
         os.environ.setdefault("HSA_ENABLE_IPC_MODE_LEGACY", "0")
-        # RCCL's kernels on a high-priority stream: a hardware queue of their own (never the main stream's) and first
-        # pick of the CUs, so a bucket's all-reduce proceeds under the backward instead of behind it
-        opts = dist.ProcessGroupNCCL.Options(is_high_priority_stream=True)
-        dist.init_process_group("nccl", device_id=torch.device("cuda", local_rank), pg_options=opts)
+        # every stream at the default priority: work on streams of different priorities can hang
+        dist.init_process_group("nccl", device_id=torch.device("cuda", local_rank))
     assert world == args.gpus, f"--gpus {args.gpus} but WORLD_SIZE={world}"
 
     from vita_amd import nn as vnn, ops

@@ -4,7 +4,7 @@ R=${GRAFT_REPO_ROOT:-$PWD}
 mode=$1; shift
 if [ "$mode" = build ]; then
   for n in "$@"; do
-    /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-value -DATT_DBG=$n -c $R/vita_amd/csrc/attention.hip -o /tmp/attention_dbg$n.o &&
+    /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-value -Xclang -target-feature -Xclang -packed-fp32-ops -DATT_DBG=$n -c $R/vita_amd/csrc/attention.hip -o /tmp/attention_dbg$n.o &&
     /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC /tmp/attention_dbg$n.o $(ls $R/vita_amd/csrc/*.o | grep -v attention.o) -o $R/vita_amd/libvita_dbg$n.so || exit 1
   done
 else

@@ -5,6 +5,7 @@ ROOT = os.path.dirname(os.path.abspath(__file__))
 SO = os.path.join(ROOT, "mfma_probe.so")
 if len(sys.argv) > 1 and sys.argv[1] == "build":
     subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-shared", "-fPIC",
+                           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                            os.path.join(ROOT, "mfma_probe.hip"), "-o", SO])
     sys.exit(0)
 import torch

@@ -166,6 +166,7 @@ __global__ __launch_bounds__(256, 3) void ln_bwd_kernel(const void* __restrict__
       const int c = (i * 64 + lane) * 4;
       xh[i] = dyv[i] = f32x4{0.f, 0.f, 0.f, 0.f};
       if (c < d) {
+#pragma clang fp contract(off)                        // products rounded, then summed (the results of earlier builds)
         const f32x4 xv = *reinterpret_cast<const f32x4*>(x + row * ldx + c);
         if (dy_f32) dyv[i] = *reinterpret_cast<const f32x4*>((const float*)dy + row * lddy + c);
         else {
@@ -194,12 +195,16 @@ __global__ __launch_bounds__(256, 3) void ln_bwd_kernel(const void* __restrict__
         }
         ag[i] += dyv[i] * xh[i];
         ab[i] += dyv[i];
-        o = (dyv[i] * g[i] - c1 - xh[i] * c2) * rs;
-        if (c + 4 > d) {
+        o = dyv[i] * g[i] - c1 - xh[i] * c2;
+        {
+#pragma clang fp contract(off)                        // as above
+          o = o * rs;
+          if (c + 4 > d) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) if (c + r >= d) o[r] = 0.f;
+            for (int r = 0; r < 4; ++r) if (c + r >= d) o[r] = 0.f;
+          }
+          o += din[i];
         }
-        o += din[i];
       }
       *reinterpret_cast<f32x4*>(dx_out + row * lddx + c) = o;
       if (dxb && c < ld_dxb)

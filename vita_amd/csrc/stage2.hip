@@ -80,6 +80,7 @@ __global__ __launch_bounds__(256) void tab_embed_bwd_kernel(const float* __restr
   if (nc == 0) {
     float sw = 0.f, sb = 0.f;
     for (int64_t b = 0; b < B; ++b) {
+#pragma clang fp contract(off)                        // sw as a rounded product, then a sum (the results of earlier builds)
       const float g = d0[b * bs];
       sw += g * x[b * F + (f - 1)];
       sb += g;
@@ -210,7 +211,10 @@ __global__ __launch_bounds__(256) void bn_fwd_kernel(const float* __restrict__ x
   }
   if (rl == 0) {
     mean_out[c] = mean; rstd_out[c] = rstd;
-    if (run_mean) run_mean[c] = (1.f - momentum) * run_mean[c] + momentum * mean;
+    if (run_mean) {
+#pragma clang fp contract(off)                        // two rounded products, then their sum (the results of earlier builds)
+      run_mean[c] = (1.f - momentum) * run_mean[c] + momentum * mean;
+    }
     if (run_var) run_var[c] = (1.f - momentum) * run_var[c] + momentum * var * (B > 1 ? (float)B / (float)(B - 1) : 1.f);
   }
 }
@@ -257,6 +261,7 @@ __global__ __launch_bounds__(256) void bn_bwd_kernel(const float* __restrict__ d
   float sb = 0.f, sg = 0.f;
   if (on)
     for (int64_t r = rl; r < B; r += 4) {
+#pragma clang fp contract(off)                        // as above
       float dz = dy[r * D + c];
       if (relu && !(y[r * D + c] > 0.f)) dz = 0.f;
       sb += dz;
