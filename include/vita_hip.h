@@ -218,6 +218,87 @@ int vita_attn_bwd(const void* qkv, const void* o, const void* dout, const float*
                   void* dqkv, void* ws, int64_t ws_bytes, int64_t B, int64_t N, int64_t H, int64_t hd,
                   int64_t hdp, float scale, void* stream);
 
+/* ------------------------------------------------------------------ 8-bit activation checkpoints
+ * No counterpart in the reference, whose only lever on activation memory is torch.utils.checkpoint
+ * (networks/imaging_encoders.py:107-114), which computes the forward pass twice.
+ * Format: a row is cut into groups of 32 neighbouring columns (the last one may be short); a group has a scale 2^e, kept as the
+ * byte e + 127, and its values are stored as e4m3 codes (OCP: no infinities, NaN = 0x7f) of value / 2^e, rounded to nearest, ties
+ * to even.  e is the smallest integer in [-117, 119] with amax / 2^e <= 448, amax over the group's finite values; values beyond
+ * 448 * 2^119 are clamped, NaN and infinities become NaN.  code * 2^e is exact in bf16.
+ * codes q: uint8 [rows][ldq], ldq % 16 == 0, 16-byte aligned, ceil(d / 32) * 32 columns are written (codes of columns >= d are 0);
+ * scale: uint8 [rows][lds], ceil(d / 32) bytes of a row are written.  Readers take bytes 10..246, which is what the writers
+ * below produce; other bytes are read without harm, their values are not specified.
+ * d <= 2^20; empty matrices are refused.  Matrices of dtype VITA_DT_BF16 need ld % 8 == 0, fp32 ld % 4 == 0, both 16-byte
+ * alignment; columns [d, ld) of an output are written as zero, columns >= d of an input are never read. */
+int vita_act8_pack(const void* x, int32_t dtype, int64_t ldx, int64_t rows, int64_t d, void* q, int64_t ldq, void* scale,
+                   int64_t lds, void* stream);
+/* y = value, or value * gamma (+ beta) per column (gamma, beta fp32 [d] or NULL): a norm's output from its normalised rows */
+int vita_act8_unpack(const void* q, int64_t ldq, const void* scale, int64_t lds, int64_t rows, int64_t d, const float* gamma,
+                     const float* beta, void* y, int32_t y_dtype, int64_t ldy, void* stream);
+/* g = GELU(z) (exact erf, bf16 out; nn.GELU of timm Mlp) and z in 8 bits, in one pass.  z bf16 or fp32. */
+int vita_gelu_act8_fwd(const void* z, int32_t z_dtype, int64_t ldz, int64_t rows, int64_t d, void* g, int64_t ldg, void* q,
+                       int64_t ldq, void* scale, int64_t lds, void* stream);
+/* dz = dg * GELU'(value) and, when g != NULL, g = GELU(value) (the operand of the following product's weight gradient).
+ * dg, dz, g bf16; dz may be dg itself (same ld). */
+int vita_gelu_act8_bwd(const void* dg, int64_t lddg, const void* q, int64_t ldq, const void* scale, int64_t lds, int64_t rows,
+                       int64_t d, void* dz, int64_t lddz, void* g, int64_t ldg, void* stream);
+/* dw[i][j] = sum over the k rows of dy[row][i] * value[row][j]: the weight gradient of y = x W^T from x's checkpoint.
+ * dy bf16 [k][lddy] (m columns), values [k][n], dw fp32 [m][lddw].  ws: 16-byte aligned scratch of vita_act8_wgrad_ws_bytes,
+ * for this call alone. */
+int64_t vita_act8_wgrad_ws_bytes(int64_t m, int64_t n, int64_t k);
+int vita_act8_wgrad(const void* dy, int64_t lddy, const void* q, int64_t ldq, const void* scale, int64_t lds, float* dw,
+                    int64_t lddw, int64_t m, int64_t n, int64_t k, void* ws, int64_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------ residual addition + norm, with an 8-bit output
+ * s = x + res;  n = (s - mu) * rstd, rstd = 1 / sqrt(mean((s - mu)^2) + eps), mu = 0 (VITA_NORM_RMS: nn.RMSNorm) or mean(s)
+ * (VITA_NORM_LAYER: nn.LayerNorm, networks/imaging_encoders.py:41,115);  y = n * gamma (+ beta).  All in fp32; s, y and the 8-bit
+ * rows are each rounded once from it (n does not see the rounding of s).  Rows of up to 8192 columns, pads included. */
+enum { VITA_NORM_RMS = 0, VITA_NORM_LAYER = 1 };
+enum { VITA_PACK_NORMED = 0, VITA_PACK_OUTPUT = 1 };
+typedef struct vita_addnorm_fwd_desc {
+  const void* x;        /* [rows][ldx], x_dtype */
+  const void* res;      /* [rows][ldr], res_dtype, or NULL */
+  void* sum;            /* optional s [rows][ldsum], sum_dtype (needs res; may be x or res itself where type and ld agree) */
+  const float* gamma;   /* fp32 [d], or NULL = 1 */
+  const float* beta;    /* fp32 [d], or NULL = 0 */
+  void* y;              /* optional [rows][ldy], y_dtype */
+  void* q;              /* optional 8-bit rows of n (VITA_PACK_NORMED) or y (VITA_PACK_OUTPUT) */
+  void* scale;
+  float* mean;          /* optional fp32 [rows] */
+  float* rstd;          /* optional fp32 [rows] */
+  int64_t rows, d;
+  int64_t ldx, ldr, ldsum, ldy, ldq, lds;
+  int32_t kind, pack;
+  int32_t x_dtype, res_dtype, sum_dtype, y_dtype;
+  float eps;
+} vita_addnorm_fwd_desc;
+int vita_addnorm_fwd(const vita_addnorm_fwd_desc* d, void* stream);
+
+/* dx = dx_in + rstd * (h - [mean(h): layer] - n * mean(h * n)), h = dy * gamma;  dgamma = sum_rows dy * n, dbeta = sum_rows dy
+ * (written, or ADDED to with accumulate != 0; one writer per element, fixed order).  n from the 8-bit rows (q, scale; packed as
+ * VITA_PACK_NORMED) or from the kept sum (src, mean, rstd).  dx serves x and res alike. */
+typedef struct vita_addnorm_bwd_desc {
+  const void* dy;       /* [rows][lddy], dy_dtype */
+  const void* src;      /* s [rows][ldx], src_dtype, or NULL */
+  const void* q;        /* 8-bit n, or NULL: exactly one of src and q */
+  const void* scale;
+  const float* mean;    /* fp32 [rows]; needed for VITA_NORM_LAYER from src */
+  const float* rstd;    /* fp32 [rows] */
+  const float* gamma;   /* fp32 [d], or NULL = 1 */
+  const void* dx_in;    /* optional gradient that reached s by other ways, [rows][lddx_in], dx_dtype */
+  void* dx;             /* [rows][lddx], dx_dtype; may be dx_in itself */
+  void* dx_bf16;        /* optional bf16 copy of dx, [rows][lddxb] */
+  float* dgamma;        /* optional fp32 [d] */
+  float* dbeta;         /* optional fp32 [d] (layer) */
+  float* partial;       /* scratch fp32 [2][vita_addnorm_bwd_nblk(rows, d)][d] when dgamma or dbeta is given, else NULL */
+  int64_t rows, d;
+  int64_t lddy, ldx, ldq, lds, lddx_in, lddx, lddxb;
+  int32_t kind, accumulate;
+  int32_t dy_dtype, src_dtype, dx_dtype;
+} vita_addnorm_bwd_desc;
+int64_t vita_addnorm_bwd_nblk(int64_t rows, int64_t d);
+int vita_addnorm_bwd(const vita_addnorm_bwd_desc* d, void* stream);
+
 /* ------------------------------------------------------------------ losses
  * CLIPLoss.forward (utils/clip_loss.py:27-40), kept in fp32:
  *   F.normalize(x, dim=1) (eps 1e-12)           -> vita_l2_normalize_fwd / _bwd

@@ -30,6 +30,24 @@ class GemmDesc(C.Structure):
     ]
 
 
+class AddNormFwdDesc(C.Structure):
+    _fields_ = [
+        ("x", vp), ("res", vp), ("sum", vp), ("gamma", vp), ("beta", vp), ("y", vp), ("q", vp), ("scale", vp), ("mean", vp),
+        ("rstd", vp), ("rows", i64), ("d", i64),
+        ("ldx", i64), ("ldr", i64), ("ldsum", i64), ("ldy", i64), ("ldq", i64), ("lds", i64),
+        ("kind", i32), ("pack", i32), ("x_dtype", i32), ("res_dtype", i32), ("sum_dtype", i32), ("y_dtype", i32), ("eps", f32),
+    ]
+
+
+class AddNormBwdDesc(C.Structure):
+    _fields_ = [
+        ("dy", vp), ("src", vp), ("q", vp), ("scale", vp), ("mean", vp), ("rstd", vp), ("gamma", vp), ("dx_in", vp), ("dx", vp),
+        ("dx_bf16", vp), ("dgamma", vp), ("dbeta", vp), ("partial", vp), ("rows", i64), ("d", i64),
+        ("lddy", i64), ("ldx", i64), ("ldq", i64), ("lds", i64), ("lddx_in", i64), ("lddx", i64), ("lddxb", i64),
+        ("kind", i32), ("accumulate", i32), ("dy_dtype", i32), ("src_dtype", i32), ("dx_dtype", i32),
+    ]
+
+
 # name -> argtypes (restype int unless noted).  Mirrors include/vita_hip.h one to one.
 SIGNATURES = {
     "vita_version": [],
@@ -73,11 +91,21 @@ SIGNATURES = {
     "vita_batchnorm_bwd": [vp, vp, vp, i64, i64, vp, vp, vp, i32, vp, vp, vp, vp],
     "vita_add_bias_rows": [vp, i64, i64, vp, vp],
     "vita_colsum_small_f32": [vp, i64, i64, vp, vp],
+    "vita_act8_pack": [vp, i32, i64, i64, i64, vp, i64, vp, i64, vp],
+    "vita_act8_unpack": [vp, i64, vp, i64, i64, i64, vp, vp, vp, i32, i64, vp],
+    "vita_gelu_act8_fwd": [vp, i32, i64, i64, i64, vp, i64, vp, i64, vp, i64, vp],
+    "vita_gelu_act8_bwd": [vp, i64, vp, i64, vp, i64, i64, i64, vp, i64, vp, i64, vp],
+    "vita_act8_wgrad_ws_bytes": [i64, i64, i64],
+    "vita_act8_wgrad": [vp, i64, vp, i64, vp, i64, vp, i64, i64, i64, i64, vp, i64, vp],
+    "vita_addnorm_fwd": [C.POINTER(AddNormFwdDesc), vp],
+    "vita_addnorm_bwd_nblk": [i64, i64],
+    "vita_addnorm_bwd": [C.POINTER(AddNormBwdDesc), vp],
     "vita_adam_step": [vp, vp, vp, vp, i64, f32, f32, f32, f32, f32, f32, i64, vp],
     "vita_cine_partial_floats": [i64],
     "vita_cine_prepare": [vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, vp, i64, i32, vp, vp, vp, vp],
 }
-_I64_RET = {"vita_layernorm_bwd_nblk", "vita_cine_partial_floats", "vita_attn_bwd_ws_bytes", "vita_attn_fwd_ws_bytes"}
+_I64_RET = {"vita_layernorm_bwd_nblk", "vita_cine_partial_floats", "vita_attn_bwd_ws_bytes", "vita_attn_fwd_ws_bytes",
+            "vita_act8_wgrad_ws_bytes", "vita_addnorm_bwd_nblk"}
 OPTIONAL = set()
 
 _lib = None

@@ -3,12 +3,12 @@ memory and the stream; every computation happens in libvita_hip.so."""
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
-from ._lib import GemmDesc, check
+from ._lib import AddNormBwdDesc, AddNormFwdDesc, GemmDesc, check
 
 BF16, F32 = 0, 1
 EPI_NONE, EPI_GELU, EPI_RESIDUAL, EPI_GELU_BWD = 0, 1, 2, 3
@@ -348,3 +348,264 @@ def attn_bwd(qkv, o, do, lse, dqkv, B, N, H, hd, hdp, scale, handoff=None):
     with _Timed("attn_bwd_kernels", 8.0 * B * H * N * N * hd):
         check(_lib.lib().vita_attn_bwd(qkv.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(), delta.data_ptr(),
                                        dqkv.data_ptr(), _p(ws), ws_bytes, B, N, H, hd, hdp, scale, _s()), "attn_bwd")
+
+
+# ----------------------------------------------------------------------------- 8-bit activation checkpoints, residual norms
+# Unlike the wrappers above these take ordinary 2-D tensors (rows of any stride the kernels can read) and check them: type,
+# device (the current one, whose current stream the kernels run on), last dimension contiguous, 16-byte aligned rows.
+class Act8(NamedTuple):
+    """[rows, d] values in 8 bits: e4m3 codes in groups of 32 columns with one power-of-two scale (e8m0) each.
+    value = code * scale, exact in bf16.  q float8_e4m3fn [rows, round_up(d, 32)], scale float8_e8m0fnu [rows, ceil(d / 32)]."""
+    q: torch.Tensor
+    scale: torch.Tensor
+    d: int
+
+    @staticmethod
+    def empty(rows: int, d: int, device) -> "Act8":
+        return Act8(torch.empty(rows, rup(d, 32), dtype=torch.float8_e4m3fn, device=device),
+                    torch.empty(rows, rup(d, 32) // 32, dtype=torch.float8_e8m0fnu, device=device), d)
+
+    @property
+    def nbytes(self) -> int:
+        return self.q.numel() + self.scale.numel()
+
+
+class AddNorm(NamedTuple):
+    """What addnorm_fwd made: y / sum are [rows, ld] with zero columns behind d, None where not asked for."""
+    y: Optional[torch.Tensor]
+    sum: Optional[torch.Tensor]
+    act: Optional[Act8]
+    mean: Optional[torch.Tensor]
+    rstd: torch.Tensor
+
+
+_KINDS = {"rms": 0, "layer": 1}
+_PACKS = {None: 0, "normed": 0, "output": 1}
+
+
+def _on_current_device(t, what):
+    if not t.is_cuda:
+        raise RuntimeError(f"vita_amd: {what} is on {t.device}; these operators run on an MI355X only (no CPU fallback)")
+    if t.device.index != torch.cuda.current_device():
+        raise RuntimeError(f"vita_amd: {what} is on cuda:{t.device.index} but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _mat(t, what, rows=None, d=None, dtypes=(torch.bfloat16, torch.float32)):
+    """Checks a [rows, d] matrix and returns its row stride in elements."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise ValueError(f"vita_amd: {what} must be a 2-D tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"vita_amd: {what} has dtype {t.dtype}, expected one of {[str(x) for x in dtypes]}")
+    if t.shape[0] == 0 or t.shape[1] == 0:
+        raise ValueError(f"vita_amd: {what} is empty: {tuple(t.shape)}")
+    if (rows is not None and t.shape[0] != rows) or (d is not None and t.shape[1] != d):
+        raise ValueError(f"vita_amd: {what} has shape {tuple(t.shape)}, expected {(rows, d)}")
+    _on_current_device(t, what)
+    step = 16 // t.element_size()
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"vita_amd: {what} must be contiguous along its last dimension (strides {t.stride()})")
+    ld = t.stride(0) if t.shape[0] > 1 else rup(t.shape[1], step)
+    if t.data_ptr() % 16 or ld % step or ld < t.shape[1]:
+        raise ValueError(f"vita_amd: rows of {what} must start on 16-byte boundaries and must not overlap (strides {t.stride()}, "
+                         f"address % 16 = {t.data_ptr() % 16}); pad the row length to a multiple of {step}")
+    return ld
+
+
+def _vec(t, what, n):
+    """Checks an fp32 vector of n elements (None passes)."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"vita_amd: {what} must be a contiguous float32 tensor of {n} elements, got {t.dtype} {tuple(t.shape)}")
+    _on_current_device(t, what)
+    return t.data_ptr()
+
+
+def _act(a, what, rows=None):
+    """Checks a checkpoint and returns (q pointer, ldq, scale pointer, lds)."""
+    if not isinstance(a, Act8):
+        raise TypeError(f"vita_amd: {what} must be an Act8")
+    if a.d < 1:
+        raise ValueError(f"vita_amd: {what} is empty")
+    g = rup(a.d, 32) // 32
+    for t, n, dt, name in ((a.q, 32 * g, torch.float8_e4m3fn, "codes"), (a.scale, g, torch.float8_e8m0fnu, "scales")):
+        if t.dtype != dt or t.dim() != 2 or t.shape[1] != n or t.shape[0] == 0 or t.shape[0] != (rows if rows is not None else a.q.shape[0]):
+            raise ValueError(f"vita_amd: {name} of {what} must be {dt} [{rows if rows is not None else 'rows'}, {n}], got {t.dtype} "
+                             f"{tuple(t.shape)}")
+    for t, n, name in ((a.q, 32 * g, "codes"), (a.scale, g, "scales")):
+        _on_current_device(t, f"{name} of {what}")
+        if (n > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < n):
+            raise ValueError(f"vita_amd: {name} of {what} have strides {t.stride()}")
+    ldq = a.q.stride(0) if a.q.shape[0] > 1 else 32 * g
+    if ldq % 16 or a.q.data_ptr() % 16:
+        raise ValueError(f"vita_amd: code rows of {what} must start on 16-byte boundaries")
+    return a.q.data_ptr(), ldq, a.scale.data_ptr(), a.scale.stride(0) if a.scale.shape[0] > 1 else g
+
+
+def _ld_out(ld, d, step, what):
+    ld = rup(d, step) if ld is None else int(ld)
+    if ld < d or ld % step:
+        raise ValueError(f"vita_amd: {what} = {ld} must be a multiple of {step} and at least {d}")
+    return ld
+
+
+def act8_pack(x) -> Act8:
+    """x bf16 | fp32 [rows, d] -> its 8-bit checkpoint."""
+    ld = _mat(x, "x")
+    rows, d = x.shape
+    a = Act8.empty(rows, d, x.device)
+    check(_lib.lib().vita_act8_pack(x.data_ptr(), _dt(x), ld, rows, d, *_act(a, "the checkpoint"), _s()), "act8_pack")
+    return a
+
+
+def act8_unpack(act: Act8, gamma=None, beta=None, dtype=torch.bfloat16, ldo=None):
+    """The values of a checkpoint (* gamma + beta per column) as [rows, ldo], zero behind column d.  bf16 without gamma is exact."""
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"vita_amd: unsupported dtype {dtype}")
+    if beta is not None and gamma is None:
+        raise ValueError("vita_amd: beta needs gamma")
+    q = _act(act, "act")
+    rows, d = act.q.shape[0], act.d
+    ldo = _ld_out(ldo, d, 8, "ldo")
+    gp, bp = _vec(gamma, "gamma", d), _vec(beta, "beta", d)
+    y = torch.empty(rows, ldo, dtype=dtype, device=act.q.device)
+    check(_lib.lib().vita_act8_unpack(*q, rows, d, gp, bp, y.data_ptr(), _dt(y), ldo, _s()), "act8_unpack")
+    return y
+
+
+def gelu_act8_fwd(z, ldg=None):
+    """z bf16 | fp32 [rows, d] -> (GELU(z) bf16 [rows, ldg] with zero pads, the 8-bit checkpoint of z)."""
+    ld = _mat(z, "z")
+    rows, d = z.shape
+    ldg = _ld_out(ldg, d, 8, "ldg")
+    g = torch.empty(rows, ldg, dtype=torch.bfloat16, device=z.device)
+    a = Act8.empty(rows, d, z.device)
+    check(_lib.lib().vita_gelu_act8_fwd(z.data_ptr(), _dt(z), ld, rows, d, g.data_ptr(), ldg, *_act(a, "the checkpoint"), _s()),
+          "gelu_act8_fwd")
+    return g, a
+
+
+def gelu_act8_bwd(dg, act: Act8, want_g=True, ldo=None):
+    """(dg * GELU'(z) bf16 [rows, ldo], GELU(z) bf16 [rows, ldo] or None), z from its checkpoint; zero pads."""
+    q = _act(act, "act")
+    rows, d = act.q.shape[0], act.d
+    ld = _mat(dg, "dg", rows, d, (torch.bfloat16,))
+    ldo = _ld_out(ldo, d, 8, "ldo")
+    dz = torch.empty(rows, ldo, dtype=torch.bfloat16, device=dg.device)
+    g = torch.empty_like(dz) if want_g else None
+    check(_lib.lib().vita_gelu_act8_bwd(dg.data_ptr(), ld, *q, rows, d, dz.data_ptr(), ldo, _p(g), ldo if want_g else 0, _s()),
+          "gelu_act8_bwd")
+    return dz, g
+
+
+def act8_wgrad(dy, act: Act8):
+    """dW fp32 [m, d] = dy^T x over the rows, from x's checkpoint; dy bf16 [rows, m]."""
+    q = _act(act, "act")
+    k, n = act.q.shape[0], act.d
+    m = dy.shape[-1]
+    ld = _mat(dy, "dy", k, m, (torch.bfloat16,))
+    dw = torch.empty(m, n, dtype=torch.float32, device=dy.device)
+    ws_bytes = _lib.lib().vita_act8_wgrad_ws_bytes(m, n, k)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device) if ws_bytes else None
+    with _Timed("act8_wgrad", 2.0 * m * n * k):
+        check(_lib.lib().vita_act8_wgrad(dy.data_ptr(), ld, *q, dw.data_ptr(), n, m, n, k, _p(ws), ws_bytes, _s()), "act8_wgrad")
+    return dw
+
+
+def addnorm_fwd(x, gamma=None, beta=None, residual=None, kind="rms", eps=1e-6, y_dtype=torch.bfloat16, sum_dtype=None, pack=None,
+                ldy=None) -> AddNorm:
+    """Norm of x (+ residual) over the last dimension, kind "rms" or "layer": y_dtype bf16 | fp32 | None, sum_dtype to also get the
+    sum, pack "normed" (the rows before gamma: addnorm_bwd's source) or "output" (y itself) for an 8-bit copy."""
+    if kind not in _KINDS or pack not in _PACKS:
+        raise ValueError(f"vita_amd: kind {kind!r} / pack {pack!r}: expected kind in {list(_KINDS)}, pack in {list(_PACKS)}")
+    if beta is not None and gamma is None:
+        raise ValueError("vita_amd: beta needs gamma")
+    if sum_dtype is not None and residual is None:
+        raise ValueError("vita_amd: sum_dtype needs a residual")
+    if y_dtype is None and pack is None:
+        raise ValueError("vita_amd: nothing to compute (no y, no pack)")
+    for t in (y_dtype, sum_dtype):
+        if t not in (None, torch.bfloat16, torch.float32):
+            raise TypeError(f"vita_amd: unsupported dtype {t}")
+    c = AddNormFwdDesc()
+    c.ldx = _mat(x, "x")
+    rows, d = x.shape
+    dev = x.device
+    c.x, c.x_dtype, c.rows, c.d = x.data_ptr(), _dt(x), rows, d
+    if residual is not None:
+        c.ldr = _mat(residual, "residual", rows, d)
+        c.res, c.res_dtype = residual.data_ptr(), _dt(residual)
+    c.gamma, c.beta = _vec(gamma, "gamma", d), _vec(beta, "beta", d)
+    c.kind, c.eps, c.pack = _KINDS[kind], eps, _PACKS[pack]
+    ld = _ld_out(ldy, d, 8, "ldy")
+    y = s = a = mean = None
+    if y_dtype is not None:
+        y = torch.empty(rows, ld, dtype=y_dtype, device=dev)
+        c.y, c.y_dtype, c.ldy = y.data_ptr(), _dt(y), ld
+    if sum_dtype is not None:
+        s = torch.empty(rows, ld, dtype=sum_dtype, device=dev)
+        c.sum, c.sum_dtype, c.ldsum = s.data_ptr(), _dt(s), ld
+    if pack is not None:
+        a = Act8.empty(rows, d, dev)
+        c.q, c.ldq, c.scale, c.lds = _act(a, "the checkpoint")
+    rstd = torch.empty(rows, dtype=torch.float32, device=dev)
+    if kind == "layer":
+        mean = torch.empty(rows, dtype=torch.float32, device=dev)
+        c.mean = mean.data_ptr()
+    c.rstd = rstd.data_ptr()
+    check(_lib.lib().vita_addnorm_fwd(C.byref(c), _s()), "addnorm_fwd")
+    return AddNorm(y, s, a, mean, rstd)
+
+
+def addnorm_bwd(dy, src, rstd, gamma=None, kind="rms", mean=None, dx_in=None, dx_dtype=torch.float32, lddx=None, want_bf16=False,
+                want_dgamma=True, want_dbeta=None, acc=None):
+    """(dx [rows, lddx], dgamma, dbeta) of addnorm_fwd; src = its Act8 ("normed") or its sum (then with mean for "layer").
+    dx is the gradient of x and of the residual, dx_in [rows, d] of type dx_dtype is added to it.  want_bf16: dx becomes the pair
+    (dx, bf16 copy).  acc = (dgamma_buf, dbeta_buf or None): fp32 [d] buffers the sums are ADDED to; None is returned for them."""
+    if kind not in _KINDS:
+        raise ValueError(f"vita_amd: kind {kind!r}: expected one of {list(_KINDS)}")
+    if dx_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"vita_amd: unsupported dtype {dx_dtype}")
+    c = AddNormBwdDesc()
+    if isinstance(src, Act8):
+        c.q, c.ldq, c.scale, c.lds = _act(src, "src")
+        rows, d = src.q.shape[0], src.d
+    else:
+        c.ldx = _mat(src, "src")
+        rows, d = src.shape
+        c.src, c.src_dtype = src.data_ptr(), _dt(src)
+        if kind == "layer" and mean is None:
+            raise ValueError("vita_amd: the layer norm's gradient from the sum needs mean")
+        c.mean = _vec(mean, "mean", rows) if kind == "layer" else None
+    dev = rstd.device
+    c.lddy = _mat(dy, "dy", rows, d)
+    c.dy, c.dy_dtype, c.rows, c.d = dy.data_ptr(), _dt(dy), rows, d
+    c.rstd, c.gamma, c.kind = _vec(rstd, "rstd", rows), _vec(gamma, "gamma", d), _KINDS[kind]
+    ld = _ld_out(lddx, d, 8, "lddx")
+    dx = torch.empty(rows, ld, dtype=dx_dtype, device=dev)
+    c.dx, c.dx_dtype, c.lddx = dx.data_ptr(), _dt(dx), ld
+    if dx_in is not None:
+        c.lddx_in = _mat(dx_in, "dx_in", rows, d, (dx_dtype,))
+        c.dx_in = dx_in.data_ptr()
+    dxb = None
+    if want_bf16:
+        dxb = torch.empty(rows, ld, dtype=torch.bfloat16, device=dev)
+        c.dx_bf16, c.lddxb = dxb.data_ptr(), ld
+    dgamma = dbeta = None
+    if acc is not None:
+        dg, db = acc
+        c.accumulate = 1
+    else:
+        want_dbeta = kind == "layer" if want_dbeta is None else want_dbeta
+        dg = dgamma = torch.empty(d, dtype=torch.float32, device=dev) if want_dgamma else None
+        db = dbeta = torch.empty(d, dtype=torch.float32, device=dev) if want_dbeta else None
+    if kind == "rms" and db is not None:
+        raise ValueError("vita_amd: the rms norm has no beta")
+    c.dgamma, c.dbeta = _vec(dg, "dgamma", d), _vec(db, "dbeta", d)
+    partial = None
+    if dg is not None or db is not None:
+        nblk = _lib.lib().vita_addnorm_bwd_nblk(rows, d)
+        partial = torch.empty(2 * nblk * d, dtype=torch.float32, device=dev)
+        c.partial = partial.data_ptr()
+    check(_lib.lib().vita_addnorm_bwd(C.byref(c), _s()), "addnorm_bwd")
+    return (dx, dxb) if want_bf16 else dx, dgamma, dbeta
