@@ -243,11 +243,12 @@ int vita_gelu_act8_fwd(const void* z, int32_t z_dtype, int64_t ldz, int64_t rows
 int vita_gelu_act8_bwd(const void* dg, int64_t lddg, const void* q, int64_t ldq, const void* scale, int64_t lds, int64_t rows,
                        int64_t d, void* dz, int64_t lddz, void* g, int64_t ldg, void* stream);
 /* dw[i][j] = sum over the k rows of dy[row][i] * value[row][j]: the weight gradient of y = x W^T from x's checkpoint.
- * dy bf16 [k][lddy] (m columns), values [k][n], dw fp32 [m][lddw].  ws: 16-byte aligned scratch of vita_act8_wgrad_ws_bytes,
+ * dy bf16 [k][lddy] (m columns), values [k][n], dw fp32 [m][lddw], written, or ADDED to with accumulate != 0
+ * (one writer per element, fixed order of summation).  ws: 16-byte aligned scratch of vita_act8_wgrad_ws_bytes,
  * for this call alone. */
 int64_t vita_act8_wgrad_ws_bytes(int64_t m, int64_t n, int64_t k);
 int vita_act8_wgrad(const void* dy, int64_t lddy, const void* q, int64_t ldq, const void* scale, int64_t lds, float* dw,
-                    int64_t lddw, int64_t m, int64_t n, int64_t k, void* ws, int64_t ws_bytes, void* stream);
+                    int64_t lddw, int64_t m, int64_t n, int64_t k, int32_t accumulate, void* ws, int64_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------ residual addition + norm, with an 8-bit output
  * s = x + res;  n = (s - mu) * rstd, rstd = 1 / sqrt(mean((s - mu)^2) + eps), mu = 0 (VITA_NORM_RMS: nn.RMSNorm) or mean(s)

@@ -87,7 +87,7 @@ def test_c_entries_refuse_before_any_launch():
     gb = lambda dg=p, ldd=64, q=p, ldq=64, s=p, lds=2, rows=4, d=64, dz=p, ldz=64, g=None, ldg=0: L.vita_gelu_act8_bwd(dg, ldd, q, ldq, s, lds, rows, d, dz, ldz, g, ldg, None)
     for kw in (dict(dg=0), dict(dz=0), dict(ldd=60), dict(g=p, ldg=32), dict(d=0)):
         assert gb(**kw) == -1, kw
-    wg = lambda dy=p, ldy=64, q=p, ldq=64, s=p, lds=2, dw=p, ldw=64, m=64, n=64, k=10, ws=p, wb=1 << 30: L.vita_act8_wgrad(dy, ldy, q, ldq, s, lds, dw, ldw, m, n, k, ws, wb, None)
+    wg = lambda dy=p, ldy=64, q=p, ldq=64, s=p, lds=2, dw=p, ldw=64, m=64, n=64, k=10, ws=p, wb=1 << 30: L.vita_act8_wgrad(dy, ldy, q, ldq, s, lds, dw, ldw, m, n, k, 0, ws, wb, None)
     for kw in (dict(dy=0), dict(ldy=60), dict(dw=0), dict(ldw=63), dict(m=0), dict(n=0), dict(k=0), dict(q=0), dict(ldq=32)):
         assert wg(**kw) == -1, kw
     need = L.vita_act8_wgrad_ws_bytes(64, 64, 10)
@@ -107,3 +107,24 @@ def test_c_entries_refuse_before_any_launch():
         assert L.vita_addnorm_bwd(C.byref(_lib.AddNormBwdDesc(**{**good, **kw})), None) == -1, kw
     assert L.vita_addnorm_bwd(C.byref(_lib.AddNormBwdDesc(**{**good, "d": 8200, "ldx": 8200, "lddx": 8200, "lddy": 8200})), None) == -2
     assert L.vita_addnorm_bwd(None, None) == -1
+
+
+def test_modules_take_and_refuse_the_new_options():
+    from torch import nn
+    from vita_amd.networks import ImagingMaskedEncoder, ViTDecoder
+    from vita_amd.nn import Block, add_rms_norm
+    b = Block(16, 2, 4.0, qkv_bias=True, norm_layer=nn.RMSNorm, saved_bits=8)
+    assert set(b.state_dict()) == {k for k in Block(16, 2, 4.0, qkv_bias=True).state_dict() if not k.startswith("norm") or k.endswith("weight")}
+    for bad in (4, "8", None):
+        with pytest.raises(ValueError):
+            Block(16, 2, 4.0, saved_bits=bad)
+    with pytest.raises(NotImplementedError):
+        Block(16, 2, 4.0, norm_layer=nn.BatchNorm1d)
+    enc = ImagingMaskedEncoder(enc_embed_dim=17, patch_size=(5, 8, 8), img_shape=[9, 10, 16, 16], enc_num_heads=1, enc_depth=2, mlp_ratio=4.0,
+                               mask_ratio=0.5, mask_type="random", use_both_axes=True, use_enc_pe=True, saved_bits=8)
+    assert all(blk.saved_bits == 8 for blk in enc.encoder)
+    assert all(blk.saved_bits == 16 for blk in ViTDecoder(16, 2, 1, 4.0).network)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        b(torch.zeros(1, 4, 16))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        add_rms_norm(torch.zeros(2, 16), None, torch.ones(16))

@@ -96,7 +96,7 @@ SIGNATURES = {
     "vita_gelu_act8_fwd": [vp, i32, i64, i64, i64, vp, i64, vp, i64, vp, i64, vp],
     "vita_gelu_act8_bwd": [vp, i64, vp, i64, vp, i64, i64, i64, vp, i64, vp, i64, vp],
     "vita_act8_wgrad_ws_bytes": [i64, i64, i64],
-    "vita_act8_wgrad": [vp, i64, vp, i64, vp, i64, vp, i64, i64, i64, i64, vp, i64, vp],
+    "vita_act8_wgrad": [vp, i64, vp, i64, vp, i64, vp, i64, i64, i64, i64, i32, vp, i64, vp],
     "vita_addnorm_fwd": [C.POINTER(AddNormFwdDesc), vp],
     "vita_addnorm_bwd_nblk": [i64, i64],
     "vita_addnorm_bwd": [C.POINTER(AddNormBwdDesc), vp],

@@ -171,28 +171,3 @@ extern "C" int vita_gelu_act8_bwd(const void* dg, int64_t lddg, const void* q, i
   VITA_CHECK_LAUNCH("vita_gelu_act8_bwd");
   return VITA_OK;
 }
-
-// ---- weight gradient dW[m][n] = sum_k dy[k][m] * value[k][n]: the values are restored as bf16 (exact) into the caller's
-// workspace and go through the bf16 matrix kernel
-extern "C" int64_t vita_act8_wgrad_ws_bytes(int64_t m, int64_t n, int64_t k) {
-  (void)m;
-  return k * ((n + 7) / 8 * 8) * 2;
-}
-extern "C" int vita_act8_wgrad(const void* dy, int64_t lddy, const void* q, int64_t ldq, const void* scale, int64_t lds, float* dw,
-                               int64_t lddw, int64_t m, int64_t n, int64_t k, void* ws, int64_t ws_bytes, void* stream) {
-  VITA_REQUIRE(m > 0 && n > 0 && k > 0 && n <= ACT8_MAX_COLS && m <= ACT8_MAX_COLS);
-  VITA_REQUIRE(act8_mat_ok(dy, lddy, m, VITA_DT_BF16) && dw && lddw >= n);
-  VITA_REQUIRE(act8_codes_ok(q, ldq, scale, lds, n));
-  VITA_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= vita_act8_wgrad_ws_bytes(m, n, k));
-  const int64_t ld = (n + 7) / 8 * 8;
-  const int rc = vita_act8_unpack(q, ldq, scale, lds, k, n, nullptr, nullptr, ws, VITA_DT_BF16, ld, stream);
-  if (rc != VITA_OK) return rc;
-  vita_gemm_desc g = {};
-  g.a = dy; g.b = ws; g.c = dw;
-  g.m = m; g.n = n; g.k = k;
-  g.lda = lddy; g.ldb = ld; g.ldc = lddw;
-  g.a_layout = g.b_layout = 1;
-  g.c_dtype = VITA_DT_F32;
-  g.alpha = 1.f;
-  return vita_gemm_bf16_ex(&g, lddw % 4 || ((uintptr_t)dw & 15) ? 1 : 0, stream);
-}

@@ -224,6 +224,8 @@ class ImagingMaskedEncoder(nn.Module):
         self.use_both_axes = kwargs.get("use_both_axes")
         self.patch_p_num = np.prod(kwargs.get("patch_size")) * self.patch_in_channels
         self.grad_checkpointing = kwargs.get("grad_checkpointing", False)
+        self.saved_bits = kwargs.get("saved_bits", 16)          # 8: activations kept for the backward pass in 8 bits
+        norm_layer = kwargs.get("norm_layer") or nn.LayerNorm
         self.pixel_unshuffle_scale = kwargs.get("pixel_unshuffle_scale")
         self.patch_embed = PatchEmbed(self.img_shape, in_channels=self.patch_in_channels,
                                       patch_size=kwargs.get("patch_size"), out_channels=kwargs.get("enc_embed_dim"))
@@ -231,9 +233,10 @@ class ImagingMaskedEncoder(nn.Module):
         self.enc_pos_embed = nn.Parameter(torch.zeros(1, 1 + self.patch_embed.num_patches, self.patch_embed.out_channels),
                                           requires_grad=False)
         self.encoder = nn.ModuleList([Block(dim=self.patch_embed.out_channels, num_heads=kwargs.get("enc_num_heads"),
-                                            mlp_ratio=kwargs.get("mlp_ratio"), qkv_bias=True)
+                                            mlp_ratio=kwargs.get("mlp_ratio"), qkv_bias=True, norm_layer=norm_layer,
+                                            saved_bits=self.saved_bits)
                                       for _ in range(kwargs.get("enc_depth"))])
-        self.encoder_norm = nn.LayerNorm(self.patch_embed.out_channels)
+        self.encoder_norm = norm_layer(self.patch_embed.out_channels)
         self.using_masker = False if kwargs.get("mask_ratio") == 0.0 else True
         if self.using_masker:
             self.masker = Masker(mask_type=kwargs.get("mask_type"), mask_ratio=kwargs.get("mask_ratio"),
@@ -285,7 +288,7 @@ class ImagingMaskedEncoder(nn.Module):
         # masked rows are never embedded: the GEMM runs on the kept tokens only (row-wise identical result)
         xp = self.patch_embed.tokens_padded(x, ids=ids, cls=self.cls_token, pos=pos)
         xp = self._run_blocks(xp)
-        return _mark(layer_norm_padded(xp, self.encoder_norm)), mask, ids_restore
+        return _mark(layer_norm_padded(xp, self.encoder_norm, self.saved_bits)), mask, ids_restore
 
     def forward(self, x):
         xp, mask, ids_restore = self.forward_padded(x)
@@ -297,15 +300,16 @@ class ImagingMaskedEncoder(nn.Module):
         xp = self.patch_embed.tokens_padded(x, ids=None, cls=self.cls_token, pos=pos)
         hidden = []
         xp = self._run_blocks(xp, collect=hidden)
-        out = _mark(layer_norm_padded(xp, self.encoder_norm))
+        out = _mark(layer_norm_padded(xp, self.encoder_norm, self.saved_bits))
         return out[..., :self.enc_embed_dim], hidden
 
 
 # ----------------------------------------------------------------------------- decoder (adjacent)
 class ViTDecoder(nn.Module):
-    def __init__(self, dim, num_heads, depth, mlp_ratio, norm_layer=nn.LayerNorm, grad_checkpointing: bool = False):
+    def __init__(self, dim, num_heads, depth, mlp_ratio, norm_layer=nn.LayerNorm, grad_checkpointing: bool = False, saved_bits: int = 16):
         super().__init__()
-        self.network = nn.ModuleList([Block(dim, num_heads, mlp_ratio, qkv_bias=True, norm_layer=norm_layer)
+        self.saved_bits = saved_bits
+        self.network = nn.ModuleList([Block(dim, num_heads, mlp_ratio, qkv_bias=True, norm_layer=norm_layer, saved_bits=saved_bits)
                                       for _ in range(depth)])
         self.norm = norm_layer(dim)
         self.grad_checkpointing = grad_checkpointing
@@ -317,7 +321,7 @@ class ViTDecoder(nn.Module):
                 xp = checkpoint(blk.forward_padded, xp, use_reentrant=False)
             else:
                 xp = blk.forward_padded(xp)
-        return _mark(layer_norm_padded(xp, self.norm))
+        return _mark(layer_norm_padded(xp, self.norm, self.saved_bits))
 
     def forward(self, x):
         return self.forward_padded(as_padded(x, self.dim, ops.rup(self.dim, 64)))[..., :self.dim]
@@ -336,7 +340,9 @@ class ImagingMaskedDecoder(nn.Module):
         self.dec_pos_embed = nn.Parameter(torch.zeros(1, 1 + self.decoder_num_patches, kwargs.get("dec_embed_dim")),
                                           requires_grad=False)
         self.decoder = ViTDecoder(dim=kwargs.get("dec_embed_dim"), num_heads=kwargs.get("dec_num_heads"),
-                                  depth=kwargs.get("dec_depth"), mlp_ratio=kwargs.get("mlp_ratio"))
+                                  depth=kwargs.get("dec_depth"), mlp_ratio=kwargs.get("mlp_ratio"),
+                                  norm_layer=kwargs.get("norm_layer") or nn.LayerNorm, saved_bits=kwargs.get("saved_bits", 16))
+        self.saved_bits = kwargs.get("saved_bits", 16)
         self.recon_head = nn.Linear(in_features=kwargs.get("dec_embed_dim"), out_features=kwargs.get("head_out_dim"))
         self.mask_token = nn.Parameter(torch.zeros(1, 1, self.dec_embed_dim), requires_grad=True)
         self.head_out_dim = int(kwargs.get("head_out_dim"))
@@ -359,7 +365,7 @@ class ImagingMaskedDecoder(nn.Module):
         De, Dd = self.enc_embed_dim, self.dec_embed_dim
         Dpe, Dpd = ops.rup(De, 64), ops.rup(Dd, 64)
         xp = as_padded(x, De, Dpe)
-        yp = linear_padded(xp, self.decoder_embed, self._sh_embed, Dpd)
+        yp = linear_padded(xp, self.decoder_embed, self._sh_embed, Dpd, self.saved_bits)
         B, n1, _ = yp.shape
         if ids_restore is not None:
             L = ids_restore.shape[1]
@@ -371,7 +377,7 @@ class ImagingMaskedDecoder(nn.Module):
             ids = torch.arange(n1, dtype=torch.int64, device=x.device).expand(B, n1)
             xp = _GatherFn.apply(yp, ids, Dd, None, self.dec_pos_embed)
         xp = self.decoder.forward_padded(xp)
-        return linear_padded(xp, self.recon_head, self._sh_head, ops.rup(self.head_out_dim, 8))
+        return linear_padded(xp, self.recon_head, self._sh_head, ops.rup(self.head_out_dim, 8), self.saved_bits)
 
     def forward(self, x, ids_restore):
         z = self.forward_logits_padded(x, ids_restore)
@@ -392,6 +398,7 @@ class TabularViT(nn.Module):
     def __init__(self, args, all_feature_names: dict, **kwargs) -> None:
         super().__init__()
         self.grad_checkpointing = args.grad_checkpointing
+        self.saved_bits = getattr(args, "saved_bits", 16)       # 8: activations kept for the backward pass in 8 bits
         self.embedding_dim = args.embedding_dim
         self.all_feature_names = all_feature_names
         self.num_numerical = len(all_feature_names["numerical"])
@@ -405,7 +412,8 @@ class TabularViT(nn.Module):
         self.cls_token = nn.Parameter(torch.zeros(1, 1, D))
         self.enc_pos_embed = nn.Parameter(torch.zeros(1, 1 + self.num_features, D), requires_grad=False)
         self.network = nn.ModuleList([Block(D, args.encoder_num_heads, args.encoder_mlp_ratio, qkv_bias=True,
-                                            norm_layer=nn.LayerNorm) for _ in range(args.encoder_num_layers)])
+                                            norm_layer=nn.LayerNorm, saved_bits=self.saved_bits)
+                                      for _ in range(args.encoder_num_layers)])
         self.norm = nn.LayerNorm(D)
         self.initialize_parameters()
 
@@ -476,7 +484,7 @@ class TabularViT(nn.Module):
                 xp = checkpoint(blk.forward_padded, xp, use_reentrant=False)
             else:
                 xp = blk.forward_padded(xp)
-        return _mark(layer_norm_padded(xp, self.norm))
+        return _mark(layer_norm_padded(xp, self.norm, self.saved_bits))
 
     def forward(self, x: torch.Tensor, num_paddings: int = None) -> torch.Tensor:
         if num_paddings is not None:

@@ -376,6 +376,16 @@ def wgrad(dy, lddy, x, ldx, rows_out, cols_out, k_tokens, row_seg=(0, 0), col_se
     return out
 
 
+def wgrad_act8(dy, act, param=None):
+    """dW = dy^T x from x's 8-bit checkpoint; ADDED to param.grad when possible (returns None then), like wgrad."""
+    tgt = grad_target(param)
+    dw = ops.act8_wgrad(dy, act, out=tgt.view(dy.shape[1], act.d) if tgt is not None else None)
+    if tgt is not None:
+        grad_done(param)
+        return None
+    return dw
+
+
 def bgrad(dy, ld, rows, cols, param=None):
     """Bias gradient = column sums of dy; accumulated into param.grad when possible (returns None then)."""
     tgt = grad_target(param)
@@ -501,18 +511,166 @@ class _BlockFn(torch.autograd.Function):
                 d_fc2w, d_fc2b)
 
 
+def norm_kind(ln):
+    """"layer" or "rms" of a Block's norm module."""
+    return "rms" if isinstance(ln, nn.RMSNorm) else "layer"
+
+
+def norm_eps(ln):
+    return torch.finfo(torch.float32).eps if ln.eps is None else ln.eps      # nn.RMSNorm(eps=None): the type's own
+
+
+def _norm_bias(ln):
+    return getattr(ln, "bias", None)         # nn.RMSNorm has none
+
+
+def norm_grad_targets(ln, need_w, need_b):
+    """(weight.grad, bias.grad or None) where the kernel may add the row sums in place, else None; cf. ln_grad_targets."""
+    b = _norm_bias(ln)
+    if b is not None:
+        return ln_grad_targets(ln, need_w, need_b)
+    gw = grad_target(ln.weight) if need_w and LN_INPLACE_GRADS else None
+    return (gw, None) if gw is not None else None
+
+
+def norm_bwd_padded(dy, src, rstd, ln, D, Dp, need_w, need_b, dx_in=None):
+    """Gradient of a norm on the padded stream from its 8-bit rows or (rms) its kept input: (dx fp32 [M, Dp], bf16 copy, dgamma, dbeta),
+    the two sums in place where the parameters allow it (None is returned for them then)."""
+    acc = norm_grad_targets(ln, need_w, need_b)
+    (dx, dxb), dw, db = ops.addnorm_bwd(dy[:, :D], src if isinstance(src, ops.Act8) else src[:, :D], rstd, ln.weight, kind=norm_kind(ln),
+                                        dx_in=None if dx_in is None else dx_in[:, :D], lddx=Dp, want_bf16=True,
+                                        want_dgamma=need_w, want_dbeta=need_b and _norm_bias(ln) is not None, acc=acc)
+    if acc is not None:
+        grad_done(ln.weight)
+        if acc[1] is not None:
+            grad_done(ln.bias)
+    return dx, dxb, dw, db
+
+
+class _BlockActFn(torch.autograd.Function):
+    """The Block with RMS norms and / or with its activations kept in 8 bits (saved_bits=8).  What the backward pass keeps of a
+    token then: the two norms' normalised rows (from which their own gradients AND the weight gradients of the products behind
+    them are computed), the MLP's pre-activation (GELU and GELU' both follow from it), all in 8 bits, and q, k, v and the
+    attention output in bf16: the backward pass recomputes the probabilities from q, k and the saved log-sum-exp, and 8-bit
+    scores would no longer sum to one against it.  About 14.5 bytes per token and channel instead of 36; the forward pass itself
+    computes with unrounded activations."""
+
+    @staticmethod
+    def forward(ctx, xp, blk, n1w, n1b, qkvw, qkvb, projw, projb, n2w, n2b, fc1w, fc1b, fc2w, fc2b):
+        dm: Dims = blk.dims
+        B, N, Dp = xp.shape
+        M, D = B * N, dm.D
+        if WGRAD_SIDE_STREAM:
+            ensure_side_stream(xp.device)
+        sh = blk.shadows()
+        x = xp.reshape(M, Dp)
+        pack = "normed" if blk.saved_bits == 8 else None
+        kind, eps = norm_kind(blk.norm1), norm_eps(blk.norm1)
+        a1 = ops.addnorm_fwd(x[:, :D], n1w, n1b, kind=kind, eps=eps, pack=pack, ldy=Dp)
+        qkv = torch.empty(M, dm.QKV, dtype=torch.bfloat16, device=x.device)
+        ops.gemm(a1.y, sh["qkv_w"], qkv, M, dm.QKV, Dp, Dp, Dp, dm.QKV, bias=sh["qkv_b"], flops=6.0 * M * D * D)
+        o, att_saved = attention_fwd(qkv, B, N, dm, DEFAULT_FLASH if blk.use_flash is None else blk.use_flash)
+        x1 = torch.empty(M, Dp, dtype=torch.float32, device=x.device)
+        ops.gemm(o, sh["proj_w"], x1, M, Dp, dm.AO, dm.AO, dm.AO, Dp, bias=sh["proj_b"], epilogue=ops.EPI_RESIDUAL,
+                 aux_in=x, ld_aux=Dp, flops=2.0 * M * D * D)
+        a2 = ops.addnorm_fwd(x1[:, :D], n2w, n2b, kind=kind, eps=norm_eps(blk.norm2), pack=pack, ldy=Dp)
+        if pack:
+            z = torch.empty(M, dm.Hp, dtype=torch.bfloat16, device=x.device)
+            ops.gemm(a2.y, sh["fc1_w"], z, M, dm.Hp, Dp, Dp, Dp, dm.Hp, bias=sh["fc1_b"], flops=2.0 * M * D * dm.hidden)
+            g, z8 = ops.gelu_act8_fwd(z[:, :dm.hidden], ldg=dm.Hp)
+            del z
+        else:
+            u = torch.empty(M, dm.Hp, dtype=torch.bfloat16, device=x.device)
+            g = torch.empty(M, dm.Hp, dtype=torch.bfloat16, device=x.device)
+            ops.gemm(a2.y, sh["fc1_w"], g, M, dm.Hp, Dp, Dp, Dp, dm.Hp, bias=sh["fc1_b"], epilogue=ops.EPI_GELU, aux_out=u,
+                     flops=2.0 * M * D * dm.hidden)
+        x2 = torch.empty(M, Dp, dtype=torch.float32, device=x.device)
+        ops.gemm(g, sh["fc2_w"], x2, M, Dp, dm.Hp, dm.Hp, dm.Hp, Dp, bias=sh["fc2_b"], epilogue=ops.EPI_RESIDUAL,
+                 aux_in=x1, ld_aux=Dp, flops=2.0 * M * D * dm.hidden)
+        ctx.blk, ctx.shape, ctx.att_mode, ctx.bits = blk, (B, N), att_saved[0], 8 if pack else 16
+        if pack:
+            ctx.save_for_backward(a1.act.q, a1.act.scale, a1.rstd, qkv, o, a2.act.q, a2.act.scale, a2.rstd, z8.q, z8.scale,
+                                  n1w, n1b, n2w, n2b, att_saved[1])
+        else:
+            ctx.save_for_backward(x, a1.rstd, a1.y, qkv, o, x1, a2.rstd, a2.y, u, g, n1w, n1b, n2w, n2b, att_saved[1])
+        return x2.view(B, N, Dp)
+
+    @staticmethod
+    def backward(ctx, dx2):
+        blk = ctx.blk
+        dm: Dims = blk.dims
+        B, N = ctx.shape
+        M, Dp, D = B * N, dm.Dp, dm.D
+        saved = ctx.saved_tensors
+        n1w, n1b, n2w, n2b, att_t = saved[10:]
+        if ctx.bits == 8:
+            q1, s1, rstd1, qkv, o, q2, s2, rstd2, qz, sz = saved[:10]
+            src1, src2, z8 = ops.Act8(q1, s1, D), ops.Act8(q2, s2, D), ops.Act8(qz, sz, dm.hidden)
+        else:
+            src1, rstd1, ln1, qkv, o, src2, rstd2, ln2, u, g = saved[:10]
+        dev = qkv.device
+        sh = blk.shadows()
+        dyb = bf16_twin(dx2, M, Dp)
+        dx2 = dx2.contiguous().view(M, Dp)
+        if dyb is None:
+            dyb = ops.cast_bf16(dx2, Dp, M, D, Dp)
+        side = _SideStream(dev)
+        need = ctx.needs_input_grad
+        a, mlp = blk.attn, blk.mlp
+        du = torch.empty(M, dm.Hp, dtype=torch.bfloat16, device=dev)
+        if ctx.bits == 8:
+            ops.gemm(dyb, sh["fc2_w"], du, M, dm.Hp, Dp, Dp, dm.Hp, dm.Hp, b_layout=1, flops=2.0 * M * D * dm.hidden)
+            du, g = ops.gelu_act8_bwd(du[:, :dm.hidden], z8, want_g=need[12], ldo=dm.Hp)
+        else:
+            ops.gemm(dyb, sh["fc2_w"], du, M, dm.Hp, Dp, Dp, dm.Hp, dm.Hp, b_layout=1, epilogue=ops.EPI_GELU_BWD, aux_in=u,
+                     ld_aux=dm.Hp, flops=2.0 * M * D * dm.hidden)
+        d_fc2w = side(wgrad, dyb, Dp, g, dm.Hp, D, dm.hidden, M, param=mlp.fc2.weight) if need[12] else None
+        d_fc2b = side(bgrad, dyb, Dp, M, D, param=mlp.fc2.bias) if need[13] else None
+        if ctx.bits == 8:        # the products' operands, restored beside the dgrad chain
+            ln2 = side(ops.act8_unpack, src2, n2w, n2b, ldo=Dp) if need[10] else None
+        d_fc1w = side(wgrad, du, dm.Hp, ln2, Dp, dm.hidden, D, M, param=mlp.fc1.weight) if need[10] else None
+        d_fc1b = side(bgrad, du, dm.Hp, M, dm.hidden, param=mlp.fc1.bias) if need[11] else None
+        dln2 = torch.empty(M, Dp, dtype=torch.bfloat16, device=dev)
+        ops.gemm(du, sh["fc1_w"], dln2, M, Dp, dm.Hp, dm.Hp, Dp, Dp, b_layout=1, flops=2.0 * M * D * dm.hidden)
+        dx1, dx1b, d_n2w, d_n2b = norm_bwd_padded(dln2, src2, rstd2, blk.norm2, D, Dp, need[8], need[9], dx_in=dx2)
+        d_projw = side(wgrad, dx1b, Dp, o, dm.AO, D, D, M, col_seg=(dm.hdp, dm.hd), n_phys=dm.AO, param=a.proj.weight) \
+            if need[6] else None
+        d_projb = side(bgrad, dx1b, Dp, M, D, param=a.proj.bias) if need[7] else None
+        do = torch.empty(M, dm.AO, dtype=torch.bfloat16, device=dev)
+        ops.gemm(dx1b, sh["proj_w"], do, M, dm.AO, Dp, Dp, dm.AO, dm.AO, b_layout=1, flops=2.0 * M * D * D)
+        dqkv = attention_bwd(do, qkv, o, (ctx.att_mode, att_t), B, N, dm)
+        if ctx.bits == 8:
+            ln1 = side(ops.act8_unpack, src1, n1w, n1b, ldo=Dp) if need[4] else None
+        d_qkvw = side(wgrad, dqkv, dm.QKV, ln1, Dp, 3 * D, D, M, row_seg=(dm.hdp, dm.hd), m_phys=dm.QKV, param=a.qkv.weight) \
+            if need[4] else None
+        d_qkvb = None
+        if a.qkv.bias is not None and need[5]:
+            d_qkvb = side(lambda: ops.unpack_vec(ops.colsum(dqkv, dm.QKV, M, dm.QKV), 3 * D, seg=(dm.hdp, dm.hd)))
+        dln1 = torch.empty(M, Dp, dtype=torch.bfloat16, device=dev)
+        ops.gemm(dqkv, sh["qkv_w"], dln1, M, Dp, dm.QKV, dm.QKV, Dp, Dp, b_layout=1, flops=6.0 * M * D * D)
+        dx, dxb, d_n1w, d_n1b = norm_bwd_padded(dln1, src1, rstd1, blk.norm1, D, Dp, need[2], need[3], dx_in=dx1)
+        side.join()
+        return (with_bf16_twin(dx.view(B, N, Dp), dxb), None, d_n1w, d_n1b, d_qkvw, d_qkvb, d_projw, d_projb, d_n2w, d_n2b, d_fc1w,
+                d_fc1b, d_fc2w, d_fc2b)
+
+
 class Block(nn.Module):
     """Drop-in for ``timm.models.vision_transformer.Block`` (0.6.12): same constructor, attribute and
-    state_dict key names (norm1, attn.qkv, attn.proj, norm2, mlp.fc1, mlp.fc2).  Only the configuration
-    the reference uses is implemented (no dropout / layer-scale / drop-path, exact-erf GELU, LayerNorm)."""
+    state_dict key names (norm1, attn.qkv, attn.proj, norm2, mlp.fc1, mlp.fc2).  The configuration the reference
+    uses (no dropout / layer-scale / drop-path, exact-erf GELU, LayerNorm), and beyond it:
+      norm_layer=nn.RMSNorm  root-mean-square norms
+      saved_bits=8           activations kept for the backward pass in 8 bits (_BlockActFn); 16 keeps them as computed"""
 
     def __init__(self, dim, num_heads, mlp_ratio=4., qkv_bias=False, drop=0., attn_drop=0., init_values=None,
-                 drop_path=0., act_layer=nn.GELU, norm_layer=nn.LayerNorm):
+                 drop_path=0., act_layer=nn.GELU, norm_layer=nn.LayerNorm, saved_bits=16):
         super().__init__()
         if drop or attn_drop or drop_path or init_values is not None:
             raise NotImplementedError("vita_amd.Block: dropout / layer-scale / drop-path are not used by ViTa")
-        if act_layer is not nn.GELU or norm_layer is not nn.LayerNorm:
-            raise NotImplementedError("vita_amd.Block: only nn.GELU + nn.LayerNorm (the reference configuration)")
+        if act_layer is not nn.GELU or norm_layer not in (nn.LayerNorm, nn.RMSNorm):
+            raise NotImplementedError("vita_amd.Block: only nn.GELU and nn.LayerNorm (the reference configuration) or nn.RMSNorm")
+        if saved_bits not in (8, 16):
+            raise ValueError(f"vita_amd.Block: saved_bits={saved_bits!r}, expected 8 or 16")
+        self.saved_bits = saved_bits
         hidden = int(dim * mlp_ratio)
         self.norm1 = norm_layer(dim)
         self.attn = Attention(dim, num_heads, qkv_bias)
@@ -545,9 +703,10 @@ class Block(nn.Module):
     def forward_padded(self, xp: torch.Tensor) -> torch.Tensor:
         """xp fp32 [B,N,Dp] contiguous with zero pads -> same layout."""
         a, m = self.attn, self.mlp
-        return _BlockFn.apply(xp, self, self.norm1.weight, self.norm1.bias, a.qkv.weight, a.qkv.bias, a.proj.weight,
-                              a.proj.bias, self.norm2.weight, self.norm2.bias, m.fc1.weight, m.fc1.bias, m.fc2.weight,
-                              m.fc2.bias)
+        fn = _BlockFn if self.saved_bits == 16 and isinstance(self.norm1, nn.LayerNorm) else _BlockActFn
+        return fn.apply(xp, self, self.norm1.weight, _norm_bias(self.norm1), a.qkv.weight, a.qkv.bias, a.proj.weight,
+                        a.proj.bias, self.norm2.weight, _norm_bias(self.norm2), m.fc1.weight, m.fc1.bias, m.fc2.weight,
+                        m.fc2.bias)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         _require_cuda(x)
@@ -588,15 +747,124 @@ class _LayerNormFn(torch.autograd.Function):
         return with_bf16_twin(dx.view(B, N, Dp), dxb), dw, db, None, None, None
 
 
-def layer_norm_padded(xp, ln: nn.LayerNorm):
-    return _LayerNormFn.apply(xp, ln.weight, ln.bias, ln.eps, ln.normalized_shape[0], ln)
+class _NormActFn(torch.autograd.Function):
+    """A norm on the padded stream with RMS norms and / or its normalised rows kept in 8 bits instead of its fp32 input."""
+
+    @staticmethod
+    def forward(ctx, xp, w, b, ln, saved_bits):
+        B, N, Dp = xp.shape
+        D = ln.normalized_shape[0]
+        x = xp.reshape(B * N, Dp)
+        a = ops.addnorm_fwd(x[:, :D], w, b, kind=norm_kind(ln), eps=norm_eps(ln), y_dtype=torch.float32,
+                            pack="normed" if saved_bits == 8 else None, ldy=Dp)
+        ctx.ln, ctx.bits = ln, saved_bits
+        if saved_bits == 8:
+            ctx.save_for_backward(a.act.q, a.act.scale, a.rstd)
+        else:
+            ctx.save_for_backward(x, a.rstd)
+        return a.y.view(B, N, Dp)
+
+    @staticmethod
+    def backward(ctx, dy):
+        ln = ctx.ln
+        B, N, Dp = dy.shape
+        D = ln.normalized_shape[0]
+        *src, rstd = ctx.saved_tensors
+        dx, dxb, dw, db = norm_bwd_padded(dy.contiguous().view(B * N, Dp), ops.Act8(*src, D) if ctx.bits == 8 else src[0], rstd, ln, D,
+                                          Dp, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
+        return with_bf16_twin(dx.view(B, N, Dp), dxb), dw, db, None, None
+
+
+def layer_norm_padded(xp, ln, saved_bits=16):
+    """nn.LayerNorm or nn.RMSNorm on the padded fp32 stream [B, N, Dp]."""
+    if saved_bits == 16 and isinstance(ln, nn.LayerNorm):
+        return _LayerNormFn.apply(xp, ln.weight, ln.bias, ln.eps, ln.normalized_shape[0], ln)
+    return _NormActFn.apply(xp, ln.weight, _norm_bias(ln), ln, saved_bits)
+
+
+class _AddRmsNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, saved_bits):
+        D = x.shape[-1]
+        stream = None if residual is None else torch.promote_types(x.dtype, residual.dtype)
+        a = ops.addnorm_fwd(_aligned_rows(x), weight, residual=None if residual is None else _aligned_rows(residual), eps=eps,
+                            y_dtype=x.dtype, sum_dtype=stream, pack="normed" if saved_bits == 8 else None)
+        ctx.set_materialize_grads(False)
+        ctx.meta = (x.shape, x.dtype, None if residual is None else residual.dtype, saved_bits)
+        y = _rows_as(a.y, x.shape)
+        s = None if residual is None else _rows_as(a.sum, x.shape)
+        if saved_bits == 8:
+            ctx.save_for_backward(a.act.q, a.act.scale, a.rstd, weight)
+        else:
+            ctx.save_for_backward(x if residual is None else s, a.rstd, weight)
+        return y, s
+
+    @staticmethod
+    def backward(ctx, dy, ds):
+        shape, xt, rt, bits = ctx.meta
+        D = shape[-1]
+        *src, rstd, weight = ctx.saved_tensors
+        need_x, need_r, need_w = ctx.needs_input_grad[:3]
+        if dy is None:
+            if ds is None:
+                return None, None, None, None, None
+            return ds.to(xt) if need_x else None, ds.to(rt) if need_r else None, None, None, None
+        src = ops.Act8(*src, D) if bits == 8 else _aligned_rows(src[0], D)
+        st = xt if rt is None else torch.promote_types(xt, rt)
+        both = rt is not None and xt != rt
+        dx, dw, _ = ops.addnorm_bwd(_aligned_rows(dy), src, rstd, weight, dx_in=None if ds is None else _aligned_rows(ds), dx_dtype=st,
+                                    want_bf16=both, want_dgamma=need_w)
+        grads = {st: (dx[0] if both else dx)[:, :D].view(shape)}
+        if both:
+            grads[torch.bfloat16] = dx[1][:, :D].view(shape)
+        return grads[xt] if need_x else None, grads[rt] if need_r else None, dw.to(weight.dtype) if need_w else None, None, None
+
+
+def _rows_as(t, shape):
+    """The [rows, ld] buffer as a tensor of `shape` on the same memory, rows ld apart.  Not a view of it as autograd sees it: a
+    custom function's outputs may be written in place only if they are no views."""
+    strides, step = [1], t.stride(0)
+    for n in reversed(shape[:-1]):
+        strides.insert(0, step)
+        step *= n
+    return torch.empty(0, dtype=t.dtype, device=t.device).set_(t.untyped_storage(), 0, tuple(shape), tuple(strides))
+
+
+def _aligned_rows(t, D=None):
+    """[..., D] -> [rows, D] whose rows start on 16-byte boundaries: a view where the layout allows it, else a padded copy."""
+    D = t.shape[-1] if D is None else D
+    t2 = t.reshape(-1, t.shape[-1])[:, :D]
+    step = 16 // t.element_size()
+    if t2.data_ptr() % 16 == 0 and (D == 1 or t2.stride(1) == 1) and (t2.shape[0] == 1 or (t2.stride(0) % step == 0 and t2.stride(0) >= D)):
+        return t2
+    out = torch.zeros(t2.shape[0], ops.rup(D, 8), dtype=t.dtype, device=t.device)
+    out[:, :D] = t2
+    return out[:, :D]
+
+
+def add_rms_norm(x, residual, weight, eps=1e-6, saved_bits=16):
+    """Root-mean-square norm of x + residual over the last dimension: (y, x + residual), or y alone for residual=None.
+
+    x, residual: bf16 or fp32 [..., D] of one shape, D <= 8192; weight fp32 [D].  y has x's type, the sum the wider of the two;
+    both are rounded once from fp32.  Differentiable in all three.  saved_bits=8 keeps the normalised rows in 8 bits for the
+    backward pass (1.03 bytes per value) instead of the sum.  vita_amd.ops.addnorm_fwd also offers the output itself in 8 bits."""
+    _require_cuda(x)
+    if saved_bits not in (8, 16):
+        raise ValueError(f"vita_amd.add_rms_norm: saved_bits={saved_bits!r}, expected 8 or 16")
+    for t in (x, residual):
+        if t is not None and t.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"vita_amd.add_rms_norm: unsupported dtype {t.dtype}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"vita_amd.add_rms_norm: x {tuple(x.shape)} and residual {tuple(residual.shape)} must have one shape (no broadcasting)")
+    y, s = _AddRmsNormFn.apply(x, residual, weight, eps, saved_bits)
+    return y if residual is None else (y, s)
 
 
 class _LinearFn(torch.autograd.Function):
     """y = x W^T + b on the padded fp32 stream: [B,N,Kp] -> [B,N,Np] (bf16 MFMA, fp32 out)."""
 
     @staticmethod
-    def forward(ctx, xp, w, b, holder, Np):
+    def forward(ctx, xp, w, b, holder, Np, saved_bits=16):
         B, N, Kp = xp.shape
         M = B * N
         out_f, in_f = w.shape
@@ -605,28 +873,37 @@ class _LinearFn(torch.autograd.Function):
         xb = ops.cast_bf16(xp.reshape(M, Kp), Kp, M, in_f, Kp)
         y = torch.empty(M, Np, dtype=torch.float32, device=xp.device)
         ops.gemm(xb, ws, y, M, Np, Kp, Kp, Kp, Np, bias=bs, flops=2.0 * M * out_f * in_f)
-        ctx.save_for_backward(xb, ws)
+        ctx.bits = saved_bits
+        if saved_bits == 8:
+            a = ops.act8_pack(xp.reshape(M, Kp)[:, :in_f])
+            ctx.save_for_backward(a.q, a.scale, ws)
+        else:
+            ctx.save_for_backward(xb, ws)
         ctx.lin_w, ctx.lin_b = w, b
         ctx.dims = (B, N, Kp, Np, out_f, in_f)
         return y.view(B, N, Np)
 
     @staticmethod
     def backward(ctx, dy):
-        xb, ws = ctx.saved_tensors
+        *xs, ws = ctx.saved_tensors
         B, N, Kp, Np, out_f, in_f = ctx.dims
         M = B * N
         dy = dy.contiguous().view(M, Np)
         dyb = ops.cast_bf16(dy, Np, M, out_f, Np)
-        need = ctx.needs_input_grad            # (xp, w, b, holder, Np)
-        dw = wgrad(dyb, Np, xb, Kp, out_f, in_f, M, param=ctx.lin_w) if need[1] else None
+        need = ctx.needs_input_grad            # (xp, w, b, holder, Np, saved_bits)
+        if ctx.bits == 8:
+            dw = wgrad_act8(dyb[:, :out_f], ops.Act8(*xs, in_f), ctx.lin_w) if need[1] else None
+        else:
+            dw = wgrad(dyb, Np, xs[0], Kp, out_f, in_f, M, param=ctx.lin_w) if need[1] else None
         db = bgrad(dyb, Np, M, out_f, param=ctx.lin_b) if need[2] else None
         dx = None
         if need[0]:
             dx = torch.empty(M, Kp, dtype=torch.float32, device=dy.device)
             ops.gemm(dyb, ws, dx, M, Kp, Np, Np, Kp, Kp, b_layout=1, flops=2.0 * M * out_f * in_f)
             dx = dx.view(B, N, Kp)
-        return dx, dw, db, None, None
+        return dx, dw, db, None, None, None
 
 
-def linear_padded(xp, lin: nn.Linear, holder: _Shadows, Np: int):
-    return _LinearFn.apply(xp, lin.weight, lin.bias, holder, Np)
+def linear_padded(xp, lin: nn.Linear, holder: _Shadows, Np: int, saved_bits=16):
+    """saved_bits=8: the input is kept for the weight gradient in 8 bits."""
+    return _LinearFn.apply(xp, lin.weight, lin.bias, holder, Np, saved_bits)

@@ -498,17 +498,21 @@ def gelu_act8_bwd(dg, act: Act8, want_g=True, ldo=None):
     return dz, g
 
 
-def act8_wgrad(dy, act: Act8):
-    """dW fp32 [m, d] = dy^T x over the rows, from x's checkpoint; dy bf16 [rows, m]."""
+def act8_wgrad(dy, act: Act8, out=None):
+    """dW fp32 [m, d] = dy^T x over the rows, from x's checkpoint; dy bf16 [rows, m].  out: a contiguous fp32 [m, d] to ADD it to."""
     q = _act(act, "act")
     k, n = act.q.shape[0], act.d
     m = dy.shape[-1]
     ld = _mat(dy, "dy", k, m, (torch.bfloat16,))
-    dw = torch.empty(m, n, dtype=torch.float32, device=dy.device)
+    if out is not None and out.shape != (m, n):
+        raise ValueError(f"vita_amd: out has shape {tuple(out.shape)}, expected {(m, n)}")
+    _vec(out, "out", m * n)
+    dw = torch.empty(m, n, dtype=torch.float32, device=dy.device) if out is None else out
     ws_bytes = _lib.lib().vita_act8_wgrad_ws_bytes(m, n, k)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device) if ws_bytes else None
     with _Timed("act8_wgrad", 2.0 * m * n * k):
-        check(_lib.lib().vita_act8_wgrad(dy.data_ptr(), ld, *q, dw.data_ptr(), n, m, n, k, _p(ws), ws_bytes, _s()), "act8_wgrad")
+        check(_lib.lib().vita_act8_wgrad(dy.data_ptr(), ld, *q, dw.data_ptr(), n, m, n, k, int(out is not None), _p(ws),
+                                           ws_bytes, _s()), "act8_wgrad")
     return dw
 
 
