@@ -172,7 +172,8 @@ def test_gelu_gradient_against_differences(ops):
 
 # ------------------------------------------------------------------------------------------------ weight gradient
 @pytest.mark.parametrize("k,m,n", [(1, 1, 1), (1, 8, 33), (3, 17, 100), (64, 40, 64), (130, 129, 257), (777, 300, 129), (2048, 520, 1025),
-                                   (4100, 1025, 320), (5000, 96, 4100)])
+                                   (4100, 1025, 320), (5000, 96, 4100), (100, 4100, 4100), (2000, 3075, 1025), (9000, 40, 40), (20000, 8, 8),
+                                   (65, 4352, 4160), (300, 4400, 4000)])
 def test_wgrad(ops, k, m, n):
     x, dy = rows_of(k, n, F32, 1.0, k), rows_of(k, m, BF16, 1.0, m, junk=False)
     a = ops.act8_pack(x)

@@ -4,16 +4,27 @@
 // v_mfma_f32_16x16x32_bf16 with no rounding beyond fp32 accumulation: nothing of the restored matrix ever reaches HBM.
 //
 //   * 256 x (16 NF) x 64 tiles, 8 waves (4 x 2), the pipeline of gemm256.hip: dy goes HBM -> LDS by LDS-DMA, fragments are read
-//     with ds_read_b64_tr_b16 under the MFMAs, one barrier per K-tile.  A code tile takes the same road through registers: 16 codes
-//     and their scale byte per load, fetched a whole K-tile before they are needed, converted (16 conversions, 4 ds_write_b128 per
-//     thread and K-tile) right behind the barrier that frees their stage - before the dy DMA is issued, so that the compiler has
-//     no LDS-DMA in flight to order the writes against.
-//   * the work is one line of tiles x K-tiles, cut into as many equal pieces as there are workgroups, wherever that falls.  A
-//     weight matrix gives few tiles (1025 x 4100: 85) and a token count long sums: a cut at whole tiles leaves up to half of
-//     the chip idle in the last round.  A piece that is not a whole tile goes to the workspace as fp32; a second kernel adds a
-//     tile's pieces in their order.  One writer per element, no atomics: the same bits on every call.
+//     with ds_read_b64_tr_b16 under the MFMAs, one barrier per K-tile.  A code tile goes through registers: 16
+//     codes and their scale byte per load, fetched a whole K-tile before they are needed; behind the barrier that frees their stage
+//     they are converted and written (16 conversions, 4 ds_write_b128 per thread and K-tile) under the first matrix instructions.
+//   * a weight matrix gives few tiles (1025 x 4100: 85) and a token count long sums, so tiles are cut along the tokens (w8_plan):
+//     whole rounds of 256 tiles stay whole, of the others as many as fit are cut into `cut` equal parts, one per workgroup, and
+//     what is left over is dealt out in short pieces behind those.  Equal cuts keep the workgroups of an XCD (blockIdx % 8) on the
+//     same tokens of neighbouring tiles, whose rows of dy and codes they then share in that XCD's L2: one line of tiles x K-tiles
+//     cut into 256 equal pieces balances better by a tenth, but the pieces drift apart and 70 % of the L2 requests missed (6 TB/s
+//     from behind it; 13826 tokens, 1025 x 3075: 114 us).
+//   * a part of a tile goes to the workspace as fp32; a second kernel adds a tile's parts in their order.  One writer per
+//     element, no atomics: the same bits on every call.
+//
+// Measured (MI355X): 3776 tokens, 1025 x 4100: 44 + 15 us (join), 720 TFLOP/s without the join; 13826 tokens, 1025 x 3075: 114 + 15 us;
+// the bf16 kernel of gemm256.hip with atomics takes 85 and 131 us for the same shapes, without the pass that restores its operand.  A
+// K-tile takes 1.48 us at 208 columns: 0.87 us of matrix instructions and barriers, the rest LDS reads (+0.18) and the operands' way
+// into LDS (+0.4; no better with the loads' data in L2, without the waits for dy, with four waves of twice the rows (124 us), or with
+// the conversions later in the K-tile (121 us) or staggered between the two halves of the workgroup (137 us)).
 #include "act8.h"
 #include "gemm256.h"
+
+#define W8_WGS 256               // workgroups of a full round: one per CU
 
 struct Wgrad8Params {
   const uint16_t* dy;
@@ -24,18 +35,23 @@ struct Wgrad8Params {
   int64_t lddy, ldq, lds, lddw;
   int64_t m, n, k;
   int tiles_m, tiles_n, kt;      // kt = K-tiles of one tile
-  int pieces;                    // workgroups
-  int per_tile;                  // pieces per tile, rounded: workgroups that far apart walk over the same tokens
+  int whole;                     // tiles [0, whole) are never cut: whole / W8_WGS per workgroup
+  int cut, cut_tiles;            // tiles [whole, whole + cut_tiles) in `cut` parts each, cut_tiles * cut <= W8_WGS
+  int piece, pieces;             // the K-tiles of the other tiles, in one line, dealt out in pieces of `piece`
   int accumulate;
 };
 
-// first iteration (tile * kt + K-tile) of piece w
-__device__ __host__ __forceinline__ int64_t w8_begin(const Wgrad8Params& P, int w) {
-  return (int64_t)P.tiles_m * P.tiles_n * P.kt * w / P.pieces;
+// tile number -> (tile row, tile column): neighbours along the shorter side, so that 32 workgroups in a row touch few panels
+__device__ __forceinline__ void w8_tile(const Wgrad8Params& P, int tile, int& tm, int& tn) {
+  if (P.tiles_n <= P.tiles_m) { tm = tile / P.tiles_n; tn = tile - tm * P.tiles_n; }
+  else { tn = tile / P.tiles_m; tm = tile - tn * P.tiles_m; }
 }
-// workspace slot of the part of a tile that piece w holds: a piece has at most one that starts inside a tile (slot 0) and one
-// that starts with a tile and ends inside it (slot 1)
-__device__ __forceinline__ int64_t w8_slot(int w, bool from_start) { return 2 * (int64_t)w + (from_start ? 1 : 0); }
+// workspace slots: one for each part of a cut tile, then two for each piece (it may hold the end of one tile and the start of the next)
+__device__ __forceinline__ int64_t w8_cut_slot(const Wgrad8Params& P, int tile, int part) { return (int64_t)(tile - P.whole) * P.cut + part; }
+__device__ __forceinline__ int64_t w8_piece_slot(const Wgrad8Params& P, int piece, int second) {
+  return (int64_t)P.cut_tiles * P.cut + 2 * piece + second;
+}
+__device__ __forceinline__ int w8_cut_begin(const Wgrad8Params& P, int part) { return (int)((int64_t)P.kt * part / P.cut); }
 
 __device__ __forceinline__ uint64_t w8_uniform(uint64_t v) { return ((uint64_t)g2_sgpr((uint32_t)(v >> 32)) << 32) | g2_sgpr((uint32_t)v); }
 // descriptor of the bytes [adv, bytes) behind base, all in scalar registers
@@ -52,17 +68,17 @@ __global__ __launch_bounds__(G2_THREADS, 2) void act8_wgrad_kernel(const Wgrad8P
   const int wm = wave & 3, wn = wave >> 2;
   const int nfw = wn == 0 ? NFW : NF - NFW;
 
-  // workgroup -> piece.  Workgroups of one XCD (blockIdx % 8) get pieces per_tile apart: neighbouring tiles over the same tokens,
-  // whose rows of dy and codes they share in that XCD's L2.
-  int w;
+  // position in the order of XCDs: neighbours share an L2
+  int l;
   {
-    const int nwg = P.pieces, qd = nwg >> 3, r = nwg & 7, xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;
-    const int l = (xcd < r ? xcd * (qd + 1) : r * (qd + 1) + (xcd - r) * qd) + idx;
-    const int per = nwg / P.per_tile;
-    w = l < per * P.per_tile ? (l % per) * P.per_tile + l / per : l;
+    const int nwg = gridDim.x, qd = nwg >> 3, r = nwg & 7, xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;
+    l = (xcd < r ? xcd * (qd + 1) : r * (qd + 1) + (xcd - r) * qd) + idx;
   }
-  const int64_t it_end = w8_begin(P, w + 1);
-  int64_t it = w8_begin(P, w);
+  // this workgroup's parts, one after another: its whole tiles, its part of a cut tile, its piece (in two parts where it straddles
+  // two tiles).  step counts them.
+  const int n_whole = P.whole / W8_WGS;
+  const int first_piece = (int)gridDim.x - 1 - l;      // from the far end: the workgroups without a cut part come first
+  int step = 0;
 
   typedef G2Loader<1, BM, 8> LoaderA;
   constexpr int BOFF = LoaderA::BYTES, STAGE = BOFF + 32768;
@@ -73,12 +89,37 @@ __global__ __launch_bounds__(G2_THREADS, 2) void act8_wgrad_kernel(const Wgrad8P
   const uint32_t boff = BOFF + brow * 512 + ((bcol ^ (int)g2_f(brow)) << 5);
   const int64_t ncodes = (P.n + ACT8_GROUP - 1) / ACT8_GROUP * ACT8_GROUP;
 
-  while (it < it_end) {
-    const int tile = (int)g2_sgpr((uint32_t)(it / P.kt));
-    const int kt0 = (int)g2_sgpr((uint32_t)(it - (int64_t)tile * P.kt));
-    int nkt = P.kt - kt0;
-    if (nkt > it_end - it) nkt = (int)(it_end - it);
-    const int tm = tile / P.tiles_n, tn = tile - tm * P.tiles_n;
+  for (;; ++step) {
+    int tile, kt0, nkt;
+    int64_t slot = -1;
+    if (step < n_whole) {
+      tile = step * W8_WGS + l; kt0 = 0; nkt = P.kt;
+    } else if (step == n_whole) {
+      if (l >= P.cut_tiles * P.cut) continue;
+      const int part = l / P.cut_tiles;
+      tile = P.whole + (l - part * P.cut_tiles);
+      kt0 = w8_cut_begin(P, part);
+      nkt = w8_cut_begin(P, part + 1) - kt0;
+      if (P.cut > 1) slot = w8_cut_slot(P, tile, part);
+    } else {
+      const int second = step - n_whole - 1;
+      if (second > 1 || first_piece >= P.pieces) break;
+      const int rest = P.whole + P.cut_tiles;          // first tile of the line
+      const int64_t line = (int64_t)(P.tiles_m * P.tiles_n - rest) * P.kt;
+      int64_t a = (int64_t)first_piece * P.piece, e = a + P.piece;
+      if (e > line) e = line;
+      const int64_t border = (a / P.kt + 1) * P.kt;    // end of the tile that the piece starts in
+      if (second) a = border; else if (e > border) e = border;
+      if (a >= e) break;
+      tile = rest + (int)(a / P.kt);
+      kt0 = (int)(a % P.kt);
+      nkt = (int)(e - a);
+      slot = w8_piece_slot(P, first_piece, second);
+    }
+    tile = (int)g2_sgpr((uint32_t)tile); kt0 = (int)g2_sgpr((uint32_t)kt0); nkt = (int)g2_sgpr((uint32_t)nkt);
+    int tm, tn;
+    w8_tile(P, tile, tm, tn);
+    if (step > 0) g2_sync_all();               // every wave has read the previous part's last K-tile: the stages are free
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * (NF * 16), k0 = (int64_t)kt0 * G2_BK;
     const int64_t krows = P.k - k0 < (int64_t)nkt * G2_BK ? P.k - k0 : (int64_t)nkt * G2_BK;      // tokens of this part
 
@@ -96,33 +137,29 @@ __global__ __launch_bounds__(G2_THREADS, 2) void act8_wgrad_kernel(const Wgrad8P
     const uint64_t qbase = w8_uniform((uint64_t)(P.q + k0 * P.ldq + n0)), sbase = w8_uniform((uint64_t)(P.scale + k0 * P.lds + (n0 >> 5)));
     const uint32_t qbytes = g2_sgpr((uint32_t)((krows - 1) * P.ldq + (ncodes - n0)));
     const uint32_t sbytes = g2_sgpr((uint32_t)((krows - 1) * P.lds + ((ncodes >> 5) - (n0 >> 5))));
+    auto b_load = [&](int t, int i, u32x4& q, uint32_t& sc) {
+      const uint32_t r = (uint32_t)t * G2_BK + 32 * i;
+      const uint32_t qa = g2_sgpr(r * (uint32_t)P.ldq), sa = g2_sgpr(r * (uint32_t)P.lds);
+      q = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(w8_rsrc(qbase, qa, qbytes), qoff, 0, 0));
+      sc = __builtin_amdgcn_raw_buffer_load_b8(w8_rsrc(sbase, sa, sbytes), soff, 0, 0);
+    };
+    // 16 codes -> 16 bf16 -> LDS.  The writes are inline asm: the compiler would wait for every LDS-DMA in flight before a write of
+    // its own.  Their results are waited for with the fragment reads (lgkmcnt(0) before the barrier).
+    auto b_write = [&](int stage, int i, const u32x4& q, uint32_t sc) {
+      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+      const float s = act8_scale(sc);
+      u32x4 o[2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        o[j >> 1][2 * (j & 1)] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q[j], s, false));
+        o[j >> 1][2 * (j & 1) + 1] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q[j], s, true));
+      }
+      const uint32_t at = boff + stage * STAGE + i * 16384;
+      asm volatile("ds_write_b128 %0, %1" :: "v"(at), "v"(o[0]) : "memory");
+      asm volatile("ds_write_b128 %0, %1 offset:16" :: "v"(at), "v"(o[1]) : "memory");
+    };
     u32x4 qv[2];
     uint32_t sv[2];
-    auto b_load = [&](int t) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t r = (uint32_t)t * G2_BK + 32 * i;
-        const uint32_t qa = g2_sgpr(r * (uint32_t)P.ldq), sa = g2_sgpr(r * (uint32_t)P.lds);
-        qv[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(w8_rsrc(qbase, qa, qbytes), qoff, 0, 0));
-        sv[i] = __builtin_amdgcn_raw_buffer_load_b8(w8_rsrc(sbase, sa, sbytes), soff, 0, 0);
-      }
-    };
-    auto b_write = [&](int stage) {
-      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float s = act8_scale(sv[i]);
-        uint32_t o[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          o[2 * j] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)qv[i][j], s, false));
-          o[2 * j + 1] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)qv[i][j], s, true));
-        }
-        char* p = smem + stage * STAGE + boff + i * 16384;
-        *reinterpret_cast<u32x4*>(p) = u32x4{o[0], o[1], o[2], o[3]};
-        *reinterpret_cast<u32x4*>(p + 16) = u32x4{o[4], o[5], o[6], o[7]};
-      }
-    };
 
     f32x4 acc[4][NFW];
 #pragma unroll
@@ -149,42 +186,42 @@ __global__ __launch_bounds__(G2_THREADS, 2) void act8_wgrad_kernel(const Wgrad8P
     W8_MFMA_GROUP(j, a0, b0);                                        \
     __builtin_amdgcn_sched_barrier(0);                               \
   }
-    // K-tiles 0 and 1 (one past the end: dy arrives as zeros, the codes are taken as zeros)
-    b_load(0);
-    b_write(0);
-    b_load(1);
+    // K-tiles 0 and 1 in one memory latency (one past the end: dy arrives as zeros, the codes are taken as zeros)
     {
-      const __amdgpu_buffer_rsrc_t ra = la.rsrc(0);
+      const __amdgpu_buffer_rsrc_t ra = la.rsrc(0), rb = la.rsrc(1);
 #pragma unroll
       for (int i = 0; i < PA; ++i) la.issue(ra, true, i, smem, wave);
-    }
-    g2_sync_all();
-    b_write(1);
-    b_load(2);
-    {
-      const __amdgpu_buffer_rsrc_t ra = la.rsrc(1);
 #pragma unroll
-      for (int i = 0; i < PA; ++i) la.issue(ra, true, i, smem + STAGE, wave);
+      for (int i = 0; i < PA; ++i) la.issue(rb, true, i, smem + STAGE, wave);
+      u32x4 q1[2];
+      uint32_t s1[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) { b_load(0, i, qv[i], sv[i]); b_load(1, i, q1[i], s1[i]); }
+      __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this wave's pieces of both K-tiles of dy are in LDS
+#pragma unroll
+      for (int i = 0; i < 2; ++i) { b_write(0, i, qv[i], sv[i]); b_write(1, i, q1[i], s1[i]); b_load(2, i, qv[i], sv[i]); }
     }
+    __builtin_amdgcn_s_waitcnt(0xc07f);        // lgkmcnt(0): the codes too
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
     W8_READ_A(0, a0); W8_READ_B(0, b0, 0, NFW);
     for (int t = 0; t + 1 < nkt; ++t) {
       W8_PHASE1();
       // K-tile t+1 is complete in LDS for every wave, and every wave has read K-tile t: its stage is free for K-tile t+2
       g2_sync_all();
       fa.toggle((t & 1) ? -STAGE : STAGE); fb.toggle((t & 1) ? -STAGE : STAGE);
-      b_write(t & 1);
-      b_load(t + 3);
       const __amdgpu_buffer_rsrc_t ra = la.rsrc(t + 2);
       char* st = smem + (t & 1) * STAGE;
 #pragma unroll
       for (int j = 0; j < NFW; ++j) {
-#pragma unroll
-        for (int i = 0; i < PA; ++i)
-          if (i == j) la.issue(ra, true, i, st, wave);
-        if (j == 0) { W8_READ_A(0, a0); }
-        if (j == 1) { W8_READ_B(0, b0, 0, 3); }
-        if (j == 2) { W8_READ_B(0, b0, 3, NFW); }
         W8_MFMA_GROUP(j, a1, b1);
+        __builtin_amdgcn_sched_barrier(0);
+        // under the matrix instructions just issued: K-tile t+2's codes and dy, the fragments of K-tile t+1's first half
+        if (j < 2) { b_write(t & 1, j, qv[j], sv[j]); b_load(t + 3, j, qv[j], sv[j]); }
+        if (j < 2) { la.issue(ra, true, 2 * j, st, wave); la.issue(ra, true, 2 * j + 1, st, wave); }
+        if (j == 1) { W8_READ_A(0, a0); }
+        if (j == 2) { W8_READ_B(0, b0, 0, 4); }
+        if (j == 3) { W8_READ_B(0, b0, 4, NFW); }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -201,7 +238,7 @@ __global__ __launch_bounds__(G2_THREADS, 2) void act8_wgrad_kernel(const Wgrad8P
 
     // lane: row lane & 15, columns 4 (lane >> 4) .. + 3 of each 16 x 16 fragment
     const int cl = wn * NFW * 16 + 4 * (lane >> 4), rl = wm * 64 + (lane & 15);
-    if (nkt == P.kt) {
+    if (slot < 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int64_t row = m0 + rl + 16 * i;
@@ -218,37 +255,44 @@ __global__ __launch_bounds__(G2_THREADS, 2) void act8_wgrad_kernel(const Wgrad8P
         }
       }
     } else {
-      float* o = P.ws + w8_slot(w, kt0 == 0) * (BM * NF * 16);
+      float* o = P.ws + slot * (BM * NF * 16);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < NFW; ++j)
           if (j < nfw) *reinterpret_cast<f32x4*>(o + (rl + 16 * i) * (NF * 16) + cl + 16 * j) = acc[i][j];
     }
-    it += nkt;
-    if (it < it_end) g2_sync_all();          // every wave has read the last K-tile: the stages are free
   }
 }
 
-// adds the parts of each cut tile, in their order.  A thread owns 4 neighbouring columns of a row.
+// adds the parts of each tile that was cut, in their order: grid (tiles behind the whole ones, quads of a tile / 256); a thread owns
+// 4 neighbouring columns of a row
 __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const Wgrad8Params P, const int width) {
-  const int tile = blockIdx.x;
-  const int64_t t0 = (int64_t)tile * P.kt, t1 = t0 + P.kt;
-  const int64_t total = (int64_t)P.tiles_m * P.tiles_n * P.kt;
-  int w0 = (int)(t0 * P.pieces / total);                 // the piece that holds iteration t0
-  while (w0 + 1 < P.pieces && w8_begin(P, w0 + 1) <= t0) ++w0;
-  while (w0 > 0 && w8_begin(P, w0) > t0) --w0;
-  if (w8_begin(P, w0 + 1) >= t1) return;                 // one piece holds all of the tile: written already
-  const int quad = blockIdx.y * 256 + threadIdx.x;       // 4 columns each
+  const int tile = P.whole + blockIdx.x;
+  const int quad = blockIdx.y * 256 + threadIdx.x;
   const int per_row = width / 4;
   const int rl = quad / per_row, cl = (quad - rl * per_row) * 4;
-  if (rl >= 256) return;
-  const int tm = tile / P.tiles_n, tn = tile - tm * P.tiles_n;
+  int tm, tn;
+  w8_tile(P, tile, tm, tn);
   const int64_t row = (int64_t)tm * 256 + rl, col = (int64_t)tn * width + cl;
-  if (row >= P.m || col >= P.n) return;
+  if (rl >= 256 || row >= P.m || col >= P.n) return;
+  const int64_t slot_floats = 256 * (int64_t)width;
+  const float* p = P.ws + (int64_t)rl * width + cl;
   f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int w = w0; w < P.pieces && w8_begin(P, w) < t1; ++w)
-    s += *reinterpret_cast<const f32x4*>(P.ws + w8_slot(w, w8_begin(P, w) <= t0) * (256 * (int64_t)width) + (int64_t)rl * width + cl);
+  if (blockIdx.x < (unsigned)P.cut_tiles) {
+    if (P.cut == 1) return;                              // written already
+    p += w8_cut_slot(P, tile, 0) * slot_floats;
+#pragma unroll 8
+    for (int i = 0; i < P.cut; ++i) s += *reinterpret_cast<const f32x4*>(p + i * slot_floats);
+  } else {
+    const int64_t t0 = (int64_t)(blockIdx.x - P.cut_tiles) * P.kt, t1 = t0 + P.kt;
+    const int w0 = (int)(t0 / P.piece), w1 = (int)((t1 + P.piece - 1) / P.piece);
+    if ((int64_t)w0 * P.piece < t0) s = *reinterpret_cast<const f32x4*>(p + w8_piece_slot(P, w0, 1) * slot_floats);
+    else s = *reinterpret_cast<const f32x4*>(p + w8_piece_slot(P, w0, 0) * slot_floats);
+    p += w8_piece_slot(P, w0 + 1, 0) * slot_floats;
+#pragma unroll 8
+    for (int i = 0; i < w1 - w0 - 1; ++i) s += *reinterpret_cast<const f32x4*>(p + 2 * i * slot_floats);
+  }
   float* o = P.dw + row * P.lddw + col;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -256,40 +300,56 @@ __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const Wgrad8Params
 }
 
 // ---- host
-struct Wgrad8Plan { int nf, pieces; };
-// Tile width and number of workgroups: the longest piece in K-tiles (plus 3 of start and end) times the cost of one (its width plus
-// what a narrow tile loses), plus the parts' way through the workspace.
+struct Wgrad8Plan { int nf, grid, whole, cut, cut_tiles, piece, pieces; int64_t slots; };
+// The cheapest of the tile widths and cuts, in microseconds of the longest workgroup: K-tiles (measured 1.36 us at 128 columns, 1.48
+// at 208, 1.6 at 256), start and end of each part, and the parts' way to the workspace and back over the whole chip
+// (256 x 16 nf floats written and read at 5 TB/s) with the join's launch and the depth of its sums.
 static Wgrad8Plan w8_plan(int64_t m, int64_t n, int64_t k) {
   const int64_t tm = (m + 255) / 256, kt = (k + G2_BK - 1) / G2_BK;
-  Wgrad8Plan best = {13, 1};
+  Wgrad8Plan best = {};
   double cost = -1;
   const int cand[3] = {8, 13, 16};
   for (int c = 0; c < 3; ++c) {
     const int nf = cand[c];
-    const int64_t tiles = tm * ((n + nf * 16 - 1) / (nf * 16)), total = tiles * kt;
-    int64_t pieces = total < 256 ? total : 256;
-    const int64_t few = (total + 3) / 4;                  // at least 4 K-tiles to a piece
-    if (pieces > few) pieces = few;
-    const double x = (double)((total + pieces - 1) / pieces + 3) * (nf + 3);
-    if (cost < 0 || x < cost) { cost = x; best = {nf, (int)pieces}; }
+    const int64_t tiles = tm * ((n + nf * 16 - 1) / (nf * 16));
+    const int64_t whole = tiles / W8_WGS * W8_WGS, left = tiles - whole;
+    for (int64_t cut = 1; cut <= W8_WGS && (cut == 1 || kt / cut >= 4); ++cut) {
+      int64_t ct = W8_WGS / cut; if (ct > left) ct = left;
+      const int64_t line = (left - ct) * kt;
+      int64_t piece = (line + W8_WGS - 1) / W8_WGS;
+      if (piece < 4) piece = kt < 4 ? kt : 4;            // <= kt always: a piece lies in two tiles at most
+      const int64_t pieces = (line + piece - 1) / piece;
+      const int64_t slots = (cut > 1 ? ct * cut : 0) + (line ? pieces + (left - ct) : 0);
+      const double kt_us = nf == 8 ? 1.36 : nf == 13 ? 1.48 : 1.6;
+      const double longest = (double)(whole / W8_WGS) * (kt * kt_us + 4) + (left ? (kt + cut - 1) / cut * kt_us + 4 : 0) +
+                             (line ? piece * kt_us + 4 : 0);
+      const double depth = line ? (double)kt / piece : (double)cut;
+      const double x = longest + (slots ? 0.0065 * nf * slots + 4 + 0.1 * depth : 0);
+      if (cost < 0 || x < cost) {
+        cost = x;
+        const int64_t busy = whole ? W8_WGS : (ct * cut > pieces ? ct * cut : pieces);
+        best = {nf, (int)busy, (int)whole, (int)cut, (int)ct, (int)piece, (int)(line ? pieces : 0), ct * cut + 2 * pieces};
+        if (!line) best.slots = cut > 1 ? ct * cut : 0;
+      }
+    }
   }
   return best;
 }
 extern "C" int64_t vita_act8_wgrad_ws_bytes(int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  if (m <= 0 || n <= 0 || k <= 0 || m > ACT8_MAX_COLS || n > ACT8_MAX_COLS || k > ((int64_t)1 << 31)) return 0;
   const Wgrad8Plan p = w8_plan(m, n, k);
-  return 2 * (int64_t)p.pieces * 256 * p.nf * 16 * 4;
+  return p.slots * 256 * p.nf * 16 * 4;
 }
 
 template <int NF>
-static int w8_launch(const Wgrad8Params& P, hipStream_t s) {
+static int w8_launch(const Wgrad8Params& P, int grid, bool join, hipStream_t s) {
   constexpr int lds = 2 * (32768 + 32768);
   static VitaPerDeviceOnce once;
   vita_set_max_lds_once(once, (const void*)act8_wgrad_kernel<NF>, lds);
-  hipLaunchKernelGGL(act8_wgrad_kernel<NF>, dim3((unsigned)P.pieces), dim3(G2_THREADS), lds, s, P);
+  hipLaunchKernelGGL(act8_wgrad_kernel<NF>, dim3((unsigned)grid), dim3(G2_THREADS), lds, s, P);
   VITA_CHECK_LAUNCH("vita_act8_wgrad");
-  if (P.pieces % (P.tiles_m * P.tiles_n) == 0 ? P.pieces > P.tiles_m * P.tiles_n : true) {
-    hipLaunchKernelGGL(act8_wgrad_join_kernel, dim3((unsigned)(P.tiles_m * P.tiles_n), 256 * NF * 4 / 256), dim3(256), 0, s, P, NF * 16);
+  if (join) {
+    hipLaunchKernelGGL(act8_wgrad_join_kernel, dim3((unsigned)(P.tiles_m * P.tiles_n - P.whole), 4 * NF), dim3(256), 0, s, P, NF * 16);
     VITA_CHECK_LAUNCH("vita_act8_wgrad_join");
   }
   return VITA_OK;
@@ -300,7 +360,8 @@ extern "C" int vita_act8_wgrad(const void* dy, int64_t lddy, const void* q, int6
   VITA_REQUIRE(m > 0 && n > 0 && k > 0 && n <= ACT8_MAX_COLS && m <= ACT8_MAX_COLS && k <= ((int64_t)1 << 31));
   VITA_REQUIRE(act8_mat_ok(dy, lddy, m, VITA_DT_BF16) && dw && lddw >= n);
   VITA_REQUIRE(act8_codes_ok(q, ldq, scale, lds, n));
-  VITA_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= vita_act8_wgrad_ws_bytes(m, n, k));
+  const int64_t need = vita_act8_wgrad_ws_bytes(m, n, k);
+  VITA_REQUIRE(need == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= need));
   const Wgrad8Plan plan = w8_plan(m, n, k);
   Wgrad8Params P;
   P.dy = (const uint16_t*)dy; P.q = (const uint8_t*)q; P.scale = (const uint8_t*)scale; P.dw = dw; P.ws = (float*)ws;
@@ -309,21 +370,19 @@ extern "C" int vita_act8_wgrad(const void* dy, int64_t lddy, const void* q, int6
   const int64_t tiles_m = (m + 255) / 256, tiles_n = (n + plan.nf * 16 - 1) / (plan.nf * 16), kt = (k + G2_BK - 1) / G2_BK;
   VITA_REQUIRE(tiles_m * tiles_n < ((int64_t)1 << 30));
   P.tiles_m = (int)tiles_m; P.tiles_n = (int)tiles_n; P.kt = (int)kt;
-  P.pieces = plan.pieces;
+  P.whole = plan.whole; P.cut = plan.cut; P.cut_tiles = plan.cut_tiles; P.piece = plan.piece; P.pieces = plan.pieces;
   P.accumulate = accumulate;
   // 32-bit offsets inside a part's tokens (a part is at most kt K-tiles long, and is read up to 3 K-tiles past its end)
-  const int64_t longest = (tiles_m * tiles_n * kt + P.pieces - 1) / P.pieces;
-  const int64_t part = ((longest < kt ? longest : kt) + 4) * G2_BK;
+  const int64_t part = ((plan.whole || plan.cut == 1 ? kt : (kt + plan.cut - 1) / plan.cut) + 4) * G2_BK;
   if (part * lddy * 2 >= (int64_t)0x7fffff00ll || part * ldq >= (int64_t)0x7fffff00ll || part * lds >= (int64_t)0x7fffff00ll) {
     vita_set_error("vita_act8_wgrad: 2 GiB or more of dy or of codes in one part of the sum", hipSuccess);
     return VITA_ERR_UNSUPPORTED;
   }
-  const int64_t per = (P.pieces + tiles_m * tiles_n / 2) / (tiles_m * tiles_n);
-  P.per_tile = per < 1 ? 1 : (int)per;
+  const bool join = plan.slots > 0;
   switch (plan.nf) {
-    case 8: return w8_launch<8>(P, (hipStream_t)stream);
-    case 13: return w8_launch<13>(P, (hipStream_t)stream);
-    default: return w8_launch<16>(P, (hipStream_t)stream);
+    case 8: return w8_launch<8>(P, plan.grid, join, (hipStream_t)stream);
+    case 13: return w8_launch<13>(P, plan.grid, join, (hipStream_t)stream);
+    default: return w8_launch<16>(P, plan.grid, join, (hipStream_t)stream);
   }
 }
 template __global__ void act8_wgrad_kernel<8>(const Wgrad8Params);
