@@ -17,11 +17,6 @@
 #define ACT8_GROUP 32
 #define ACT8_MAX_COLS (1 << 20)
 
-// |v| as an ordered integer, 0 for NaN and infinities
-__device__ __forceinline__ uint32_t act8_mag(float v) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;
-}
 __device__ __forceinline__ uint32_t act8_quad_max(uint32_t v) {
   const uint32_t a = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true);    // quad_perm [1,0,3,2]
   v = v > a ? v : a;
@@ -38,18 +33,36 @@ __device__ __forceinline__ uint32_t act8_scale_byte(uint32_t amax) {
 __device__ __forceinline__ float act8_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
 __device__ __forceinline__ float act8_inv_scale(uint32_t byte) { return __builtin_bit_cast(float, (254u - byte) << 23); }
 
+// Bits of the largest magnitude whose group the plain path may code: above it lie NaN, infinities and amax > 1.75 * 2^127, where e is
+// at its end and values saturate
+#define ACT8_TOP 0x7f600000u
+
 // the 8 values of a lane (all 4 lanes of the quad call it) -> their codes; byte = the group's scale byte
 __device__ __forceinline__ u32x2 act8_encode(const float (&v)[8], uint32_t& byte) {
   uint32_t m = 0;
 #pragma unroll
-  for (int r = 0; r < 8; ++r) { const uint32_t a = act8_mag(v[r]); m = m > a ? m : a; }
-  byte = act8_scale_byte(act8_quad_max(m));
-  const float inv = act8_inv_scale(byte);
+  for (int r = 0; r < 8; ++r) { const uint32_t a = __builtin_bit_cast(uint32_t, v[r]) & 0x7fffffffu; m = m > a ? m : a; }
+  m = act8_quad_max(m);
   float t[8];
+  if (__builtin_expect(m > ACT8_TOP, 0)) {      // the four lanes of a quad together
+    m = 0;
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    t[r] = __builtin_amdgcn_fmed3f(v[r] * inv, -448.f, 448.f);
-    if ((__builtin_bit_cast(uint32_t, v[r]) & 0x7f800000u) == 0x7f800000u) t[r] = __builtin_nanf("");
+    for (int r = 0; r < 8; ++r) {
+      const uint32_t a = __builtin_bit_cast(uint32_t, v[r]) & 0x7fffffffu;
+      if (a < 0x7f800000u) m = m > a ? m : a;
+    }
+    byte = act8_scale_byte(act8_quad_max(m));
+    const float inv = act8_inv_scale(byte);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      t[r] = __builtin_amdgcn_fmed3f(v[r] * inv, -448.f, 448.f);
+      if ((__builtin_bit_cast(uint32_t, v[r]) & 0x7f800000u) == 0x7f800000u) t[r] = __builtin_nanf("");
+    }
+  } else {
+    byte = act8_scale_byte(m);
+    const float inv = act8_inv_scale(byte);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) t[r] = v[r] * inv;
   }
   u32x2 q;
 #pragma unroll
@@ -106,6 +119,17 @@ __device__ __forceinline__ void raw_values8(const Raw8& w, float (&v)[8]) {
 __device__ __forceinline__ u32x4 pack_bf16x8(const float (&v)[8]) {
   return u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
 }
+// 8 neighbouring floats of a vector of d (gamma, beta), `fill` behind its end and for NULL; al: 16-byte aligned
+__device__ __forceinline__ void vec_load8(const float* p, int c, int d, bool al, float fill, float (&v)[8]) {
+  if (p && al && c + 8 <= d) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p + c), b = *reinterpret_cast<const f32x4*>(p + c + 4);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) { v[r] = a[r]; v[4 + r] = b[r]; }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v[r] = p && c + r < d ? p[c + r] : fill;
+  }
+}
 // columns [c, c + 8) of a row of `ld` columns (ld % 8 == 0 for bf16, % 4 for fp32): all 8, or those below ld
 __device__ __forceinline__ void store8(void* row, int c, int64_t ld, bool f32, const float (&v)[8]) {
   if (f32) {
@@ -114,6 +138,31 @@ __device__ __forceinline__ void store8(void* row, int c, int64_t ld, bool f32, c
   } else if (c < ld) {
     *reinterpret_cast<u32x4*>((uint16_t*)row + c) = pack_bf16x8(v);
   }
+}
+
+// ---- one column to a lane: 64 neighbouring columns of a wave, a group is one half of it
+template <bool F32>
+__device__ __forceinline__ float load1(const void* row, int c, int d) {
+  if (c >= d) return 0.f;
+  return F32 ? ((const float*)row)[c] : bf16_bits_to_f32(((const uint16_t*)row)[c]);
+}
+__device__ __forceinline__ void store1(void* row, int c, int64_t ld, bool f32, float v) {
+  if (c >= ld) return;
+  if (f32) ((float*)row)[c] = v; else ((uint16_t*)row)[c] = f32_to_bf16_bits(v);
+}
+__device__ __forceinline__ uint8_t act8_encode1(float v, uint32_t& byte) {
+  const uint32_t a = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
+  uint32_t m = a < 0x7f800000u ? a : 0u;
+  m = act8_quad_max(m);
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) { const uint32_t b = (uint32_t)__shfl_xor((int)m, o, 64); m = m > b ? m : b; }
+  byte = act8_scale_byte(m);
+  float t = __builtin_amdgcn_fmed3f(v * act8_inv_scale(byte), -448.f, 448.f);
+  if (a >= 0x7f800000u) t = __builtin_nanf("");
+  return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(t, t, 0, false);
+}
+__device__ __forceinline__ float act8_decode1(uint8_t q, uint8_t byte) {
+  return __builtin_amdgcn_cvt_f32_fp8((int)q, 0) * act8_scale(byte);
 }
 
 // host: a [rows][ld] matrix of a VITA_DT_* type that the kernels may read / write in 16-byte pieces

@@ -68,16 +68,22 @@ extern "C" int vita_act8_pack(const void* x, int32_t dtype, int64_t ldx, int64_t
 // y = value [* gamma + beta], columns [d, ldy) zero
 __global__ __launch_bounds__(A8_THREADS) void act8_unpack_kernel(const uint8_t* __restrict__ q, int64_t ldq,
                                                                  const uint8_t* __restrict__ scale, int64_t lds, ChunkMap M, int d,
-                                                                 const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                                 const float* __restrict__ gamma, const float* __restrict__ beta, int al,
                                                                  void* __restrict__ y, int64_t ldy, int y_f32) {
   for_chunks(M, [&](int64_t row, int c) {
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (c < d) {
       act8_decode(*reinterpret_cast<const u32x2*>(q + row * ldq + c), scale[row * lds + (c >> 5)], v);
+      if (gamma) {
+        float g[8], b[8];
+        vec_load8(gamma, c, d, al, 0.f, g);
+        vec_load8(beta, c, d, al, 0.f, b);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        if (c + r >= d) v[r] = 0.f;
-        else if (gamma) v[r] = __builtin_fmaf(v[r], gamma[c + r], beta ? beta[c + r] : 0.f);
+        for (int r = 0; r < 8; ++r) v[r] = __builtin_fmaf(v[r], g[r], b[r]);
+      }
+      if (c + 8 > d) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) if (c + r >= d) v[r] = 0.f;
       }
     }
     store8((char*)y + row * ldy * (y_f32 ? 4 : 2), c, ldy, y_f32, v);
@@ -93,7 +99,7 @@ extern "C" int vita_act8_unpack(const void* q, int64_t ldq, const void* scale, i
   ChunkMap M; dim3 grid;
   VITA_REQUIRE(chunk_grid(rows, ldy, M, grid));
   hipLaunchKernelGGL(act8_unpack_kernel, grid, dim3(A8_THREADS), 0, (hipStream_t)stream, (const uint8_t*)q, ldq, (const uint8_t*)scale,
-                     lds, M, (int)d, gamma, beta, y, ldy, y_dtype == VITA_DT_F32);
+                     lds, M, (int)d, gamma, beta, (((uintptr_t)gamma | (uintptr_t)beta) & 15) == 0, y, ldy, y_dtype == VITA_DT_F32);
   VITA_CHECK_LAUNCH("vita_act8_unpack");
   return VITA_OK;
 }

@@ -7,93 +7,159 @@
 // backward, with h = dy gamma:
 //   dx = dx_in + rstd (h - [mean(h)] - n mean(h n)),  dgamma = sum_rows dy n,  dbeta = sum_rows dy
 // n comes from the 8-bit rows (1.03 bytes a value and rstd) or from s and (mu, rstd).
+//
+// Both move bytes.  Measured (MI355X, kernels alone; a copy of that size reaches 5 TB/s):
+//   forward, 46082 x 1025, bf16 + fp32 -> fp32 sum, bf16 y, 8-bit n: 134 us, 4.6 TB/s (one wave per row and a row per block of gamma
+//     and beta loads: 186 us; rows dealt to resident waves with gamma in registers: 141 us; 64 columns behind the chunks one to a
+//     lane: 134 us)
+//   backward, 13826 x 1025, from 8 bits, bf16 dy, fp32 dx_in and dx: 38 + 4 us (sums of the partial rows), 4.1 TB/s (gamma read
+//     anew for each row and dx_in after the sums: 89 + 16 us; loads together, gamma in registers: 61; 768 partial rows of 1025
+//     columns added with all loads in flight: 4 instead of 16 us; last columns one to a lane, 3 blocks a CU instead of 2: 38)
+//   backward, 4096 x 4096, from a bf16 sum: 33 + 4 us, 4.1 TB/s (62 + 13 us before)
 #include "act8.h"
 
 #define AN_RMS 0
 #define AN_LAYER 1
 #define AN_MAX_D 8192
+#define AN_FWD_MAXBLK 2048
+#define AN_FEW_ROWS 1024
 
-// sum over the W waves that share a row (W = 1: the wave itself, no barrier)
+// sums over the W waves that share a row (W = 1: the wave itself, no barrier), two at a time
 template <int W>
-__device__ __forceinline__ float row_sum(float v, float* red, int wave, int lane) {
-  v = wave_sum(v);
-  if (W == 1) return v;
-  __syncthreads();                    // the previous use of red is over
-  if (lane == 0) red[wave] = v;
-  __syncthreads();
-  float t = red[0];
+__device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2][W], int& turn, int wave, int lane) {
 #pragma unroll
-  for (int w = 1; w < W; ++w) t += red[w];
-  return t;
+  for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
+  if (W == 1) return;
+  turn ^= 1;                          // two slots in turn: the barrier of the next sum lies between a slot's reads and its next writes
+  if (lane == 0) { red[turn][0][wave] = a; red[turn][1][wave] = b; }
+  __syncthreads();
+  a = red[turn][0][0]; b = red[turn][1][0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) { a += red[turn][0][w]; b += red[turn][1][w]; }
+}
+template <int W>
+__device__ __forceinline__ float row_sum(float a, float (*red)[2][W], int& turn, int wave, int lane) {
+  a = wave_sum(a);
+  if (W == 1) return a;
+  turn ^= 1;
+  if (lane == 0) red[turn][0][wave] = a;
+  __syncthreads();
+  a = red[turn][0][0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) a += red[turn][0][w];
+  return a;
 }
 
-template <int W, int NV, bool XF, int RT>      // RT: 0 no residual, 1 bf16, 2 fp32
-__global__ __launch_bounds__(256) void addnorm_fwd_kernel(const vita_addnorm_fwd_desc D) {
-  __shared__ float red[W];
+// A wave (W = 1) or the four waves of a block (W = 4) walk over rows, 8 neighbouring columns to a lane and chunk, the row in
+// registers from its loads to its stores; gamma and beta stay in registers.  T: up to 64 columns behind the last whole chunk go one to
+// a lane instead of opening another chunk (1025 columns would fill 1 of its 64 lanes and cost every lane 8 columns of registers and
+// arithmetic; measured below).
+template <int W, int NV, bool T, bool XF, int RT>      // RT: 0 no residual, 1 bf16, 2 fp32
+__global__ __launch_bounds__(256) void addnorm_fwd_kernel(const vita_addnorm_fwd_desc D, const int al) {
+  __shared__ float red[2][2][W];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
-  if (row >= D.rows) return;          // whole rows leave together: W waves of one row share the block
   const int d = (int)D.d, t0 = (W == 1 ? lane : (int)threadIdx.x) * 8;
-  Raw8 xr[NV], rr[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) xr[i] = raw_load8<XF>((const char*)D.x + row * D.ldx * (XF ? 4 : 2), t0 + i * W * 512, d);
-  if (RT) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) rr[i] = raw_load8<RT == 2>((const char*)D.res + row * D.ldr * (RT == 2 ? 4 : 2), t0 + i * W * 512, d);
-  }
-  float v[NV][8], s = 0.f;
+  const double inv_d = 1.0 / (double)d;
+  int turn = 0;
+  float gm[NV][8], bt[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    raw_values8<XF>(xr[i], v[i]);
+    vec_load8(D.gamma, t0 + i * W * 512, d, al, 1.f, gm[i]);
+    vec_load8(D.beta, t0 + i * W * 512, d, al, 0.f, bt[i]);
+  }
+  const int ct = NV * 512 + lane;                // the lane's column behind the chunks
+  const float gt = T && ct < d && D.gamma ? D.gamma[ct] : 1.f, btt = T && ct < d && D.beta ? D.beta[ct] : 0.f;
+  const int64_t step = W == 1 ? (int64_t)gridDim.x * 4 : (int64_t)gridDim.x;
+  for (int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x; row < D.rows; row += step) {
+    Raw8 xr[NV], rr[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) xr[i] = raw_load8<XF>((const char*)D.x + row * D.ldx * (XF ? 4 : 2), t0 + i * W * 512, d);
     if (RT) {
-      float t[8];
-      raw_values8<RT == 2>(rr[i], t);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) v[i][r] += t[r];
+      for (int i = 0; i < NV; ++i) rr[i] = raw_load8<RT == 2>((const char*)D.res + row * D.ldr * (RT == 2 ? 4 : 2), t0 + i * W * 512, d);
     }
-#pragma unroll
-    for (int r = 0; r < 8; ++r) s += v[i][r];
-  }
-  if (RT && D.sum) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      store8((char*)D.sum + row * D.ldsum * (D.sum_dtype == VITA_DT_F32 ? 4 : 2), t0 + i * W * 512, D.ldsum, D.sum_dtype == VITA_DT_F32, v[i]);
-  }
-  const float inv_d = 1.f / (float)d;
-  const float mu = D.kind == AN_LAYER ? row_sum<W>(s, red, wave, lane) * inv_d : 0.f;
-  float q = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const bool on = t0 + i * W * 512 + r < d;
-      v[i][r] = on ? v[i][r] - mu : 0.f;
-      q = __builtin_fmaf(v[i][r], v[i][r], q);
+    float vt = 0.f;
+    if (T) {
+      vt = load1<XF>((const char*)D.x + row * D.ldx * (XF ? 4 : 2), ct, d);
+      if (RT) vt += load1<RT == 2>((const char*)D.res + row * D.ldr * (RT == 2 ? 4 : 2), ct, d);
     }
-  const float rs = rsqrtf(row_sum<W>(q, red, wave, lane) * inv_d + D.eps);
-  if (t0 == 0) {
-    if (D.mean) D.mean[row] = mu;
-    if (D.rstd) D.rstd[row] = rs;
-  }
-  const int dq = (d + 31) & ~31;
+    float v[NV][8], s = vt;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = t0 + i * W * 512;
-    float y[8];
+    for (int i = 0; i < NV; ++i) {
+      raw_values8<XF>(xr[i], v[i]);
+      if (RT) {
+        float t[8];
+        raw_values8<RT == 2>(rr[i], t);
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      v[i][r] *= rs;
-      y[r] = c + r < d ? __builtin_fmaf(v[i][r], D.gamma ? D.gamma[c + r] : 1.f, D.beta ? D.beta[c + r] : 0.f) : 0.f;
-    }
-    if (D.q) {
-      uint32_t byte;
-      const u32x2 w = D.pack == VITA_PACK_OUTPUT ? act8_encode(y, byte) : act8_encode(v[i], byte);
-      if (c < dq) {
-        *reinterpret_cast<u32x2*>((uint8_t*)D.q + row * D.ldq + c) = w;
-        if ((c & 31) == 0) ((uint8_t*)D.scale)[row * D.lds + (c >> 5)] = (uint8_t)byte;
+        for (int r = 0; r < 8; ++r) v[i][r] += t[r];
       }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s += v[i][r];
     }
-    if (D.y) store8((char*)D.y + row * D.ldy * (D.y_dtype == VITA_DT_F32 ? 4 : 2), c, D.ldy, D.y_dtype == VITA_DT_F32, y);
+    if (RT && D.sum) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        store8((char*)D.sum + row * D.ldsum * (D.sum_dtype == VITA_DT_F32 ? 4 : 2), t0 + i * W * 512, D.ldsum, D.sum_dtype == VITA_DT_F32, v[i]);
+      if (T) store1((char*)D.sum + row * D.ldsum * (D.sum_dtype == VITA_DT_F32 ? 4 : 2), ct, D.ldsum, D.sum_dtype == VITA_DT_F32, vt);
+    }
+    if (D.kind == AN_LAYER) {
+      const float mu = (float)(row_sum<W>(s, red, turn, wave, lane) * inv_d);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[i][r] -= mu;
+      if (T && ct < d) vt -= mu;
+      if (D.mean && t0 == 0) D.mean[row] = mu;
+    }
+    float q = T ? vt * vt : 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = t0 + i * W * 512;
+      if (c + 8 > d) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) if (c + r >= d) v[i][r] = 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) q = __builtin_fmaf(v[i][r], v[i][r], q);
+    }
+    // rstd as a pair of floats from 64 bits, n rounded once from its product: an error in the last bit of rstd would send ten times as
+    // many values across the borders of the 8-bit codes as the roundings that are left
+    const double r = 1.0 / sqrt((double)row_sum<W>(q, red, turn, wave, lane) * inv_d + (double)D.eps);
+    const float rs = (float)r, rl = (float)(r - (double)rs);
+    if (D.rstd && t0 == 0) D.rstd[row] = rs;
+    const int dq = (d + 31) & ~31;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = t0 + i * W * 512;
+      float y[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        v[i][r] = __builtin_fmaf(v[i][r], rs, v[i][r] * rl);
+        y[r] = __builtin_fmaf(v[i][r], gm[i][r], bt[i][r]);        // 0 * 1 + 0 behind the row's end
+      }
+      if (D.q) {
+        uint32_t byte;
+        const u32x2 w = D.pack == VITA_PACK_OUTPUT ? act8_encode(y, byte) : act8_encode(v[i], byte);
+        if (c < dq) {
+          *reinterpret_cast<u32x2*>((uint8_t*)D.q + row * D.ldq + c) = w;
+          if ((c & 31) == 0) ((uint8_t*)D.scale)[row * D.lds + (c >> 5)] = (uint8_t)byte;
+        }
+      }
+      if (D.y) store8((char*)D.y + row * D.ldy * (D.y_dtype == VITA_DT_F32 ? 4 : 2), c, D.ldy, D.y_dtype == VITA_DT_F32, y);
+    }
+    if (T) {
+      vt = __builtin_fmaf(vt, rs, vt * rl);
+      const float y = __builtin_fmaf(vt, gt, btt);
+      if (D.q) {
+        uint32_t byte;
+        const uint8_t w = act8_encode1(D.pack == VITA_PACK_OUTPUT ? y : vt, byte);
+        if (ct < dq) {
+          ((uint8_t*)D.q)[row * D.ldq + ct] = w;
+          if ((ct & 31) == 0) ((uint8_t*)D.scale)[row * D.lds + (ct >> 5)] = (uint8_t)byte;
+        }
+      }
+      if (D.y) store1((char*)D.y + row * D.ldy * (D.y_dtype == VITA_DT_F32 ? 4 : 2), ct, D.ldy, D.y_dtype == VITA_DT_F32, y);
+    }
   }
 }
 
@@ -121,44 +187,57 @@ extern "C" int vita_addnorm_fwd(const vita_addnorm_fwd_desc* dp, void* stream) {
   }
   VITA_REQUIRE(D.rows < (int64_t)0x7fffffff);
   const int rt = D.res ? (D.res_dtype == VITA_DT_F32 ? 2 : 1) : 0;
-#define AN_LAUNCH(W, NV, XF, RT)                                                                                                     \
-  hipLaunchKernelGGL((addnorm_fwd_kernel<W, NV, XF, RT>), dim3((unsigned)(W == 1 ? (D.rows + 3) / 4 : D.rows)), dim3(256), 0,        \
-                     (hipStream_t)stream, D)
-#define AN_TYPES(W, NV)                                                                 \
-  do {                                                                                  \
-    if (D.x_dtype == VITA_DT_F32) {                                                     \
-      if (rt == 0) AN_LAUNCH(W, NV, true, 0); else if (rt == 1) AN_LAUNCH(W, NV, true, 1); else AN_LAUNCH(W, NV, true, 2);    \
-    } else {                                                                            \
-      if (rt == 0) AN_LAUNCH(W, NV, false, 0); else if (rt == 1) AN_LAUNCH(W, NV, false, 1); else AN_LAUNCH(W, NV, false, 2); \
-    }                                                                                   \
+  const int al = (((uintptr_t)D.gamma | (uintptr_t)D.beta) & 15) == 0;
+  const auto blocks = [&](int w) { const int64_t n = w == 1 ? (D.rows + 3) / 4 : D.rows; return n < AN_FWD_MAXBLK ? n : AN_FWD_MAXBLK; };
+#define AN_LAUNCH(W, NV, T, XF, RT) \
+  hipLaunchKernelGGL((addnorm_fwd_kernel<W, NV, T, XF, RT>), dim3((unsigned)(blocks(W))), dim3(256), 0, (hipStream_t)stream, D, al)
+#define AN_TYPES(W, NV, T)                                                                                                                   \
+  do {                                                                                                                                       \
+    if (D.x_dtype == VITA_DT_F32) {                                                                                                          \
+      if (rt == 0) AN_LAUNCH(W, NV, T, true, 0); else if (rt == 1) AN_LAUNCH(W, NV, T, true, 1); else AN_LAUNCH(W, NV, T, true, 2);         \
+    } else {                                                                                                                                 \
+      if (rt == 0) AN_LAUNCH(W, NV, T, false, 0); else if (rt == 1) AN_LAUNCH(W, NV, T, false, 1); else AN_LAUNCH(W, NV, T, false, 2);      \
+    }                                                                                                                                        \
   } while (0)
-  if (width <= 512) AN_TYPES(1, 1);
-  else if (width <= 1536) AN_TYPES(1, 3);
-  else if (width <= 4096) AN_TYPES(4, 2);
-  else AN_TYPES(4, 4);
+  // few rows: four waves to a row shorten the way through one row
+  if (width <= 512) AN_TYPES(1, 1, false);
+  else if (width <= 2048 && D.rows <= AN_FEW_ROWS) AN_TYPES(4, 1, false);
+  else if (width <= 1024) AN_TYPES(1, 2, false);
+  else if (width <= 1088) AN_TYPES(1, 2, true);
+  else if (width <= 1536) AN_TYPES(1, 3, false);
+  else if (width <= 4096) AN_TYPES(4, 2, false);
+  else AN_TYPES(4, 4, false);
 #undef AN_TYPES
 #undef AN_LAUNCH
   VITA_CHECK_LAUNCH("vita_addnorm_fwd");
   return VITA_OK;
 }
 
-// ---- backward: a block walks over rows; a lane's dgamma / dbeta sums stay in registers, then one partial row per block
+// ---- backward: rows as above; every load of a row is in flight before its first sum, the values are taken from the raw registers
+// twice (to sum, to store) instead of being kept, and a lane's dgamma / dbeta sums stay in registers until one partial row per block
 #define AN_BWD_MAXBLK 768
-template <int W, int NV, int SRC, bool DYF>      // SRC: 0 8-bit rows, 1 bf16 sum, 2 fp32 sum
-__global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd_desc D, const int nblk) {
-  __shared__ float red[W == 1 ? 1 : 8];
-  __shared__ float sums[W == 1 ? NV * 512 : 1];
+template <int W, int NV, bool T, int SRC, bool DYF>      // SRC: 0 8-bit rows, 1 bf16 sum, 2 fp32 sum
+__global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd_desc D, const int al) {
+  __shared__ float red[2][2][W];
+  __shared__ __attribute__((aligned(16))) float sums[W == 1 ? NV * 512 + 64 : 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int d = (int)D.d, t0 = (W == 1 ? lane : (int)threadIdx.x) * 8;
+  const int d = (int)D.d, t0 = (W == 1 ? lane : (int)threadIdx.x) * 8, nblk = gridDim.x;
   const float inv_d = 1.f / (float)d;
-  float ag[NV][8], ab[NV][8];
+  const bool dxf = D.dx_dtype == VITA_DT_F32;
+  int turn = 0;
+  float gm[NV][8], ag[NV][8], ab[NV][8];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    vec_load8(D.gamma, t0 + i * W * 512, d, al, 1.f, gm[i]);
 #pragma unroll
     for (int r = 0; r < 8; ++r) ag[i][r] = ab[i][r] = 0.f;
+  }
+  const int ct = NV * 512 + lane;                // the lane's column behind the chunks
+  const float gt = T && ct < d && D.gamma ? D.gamma[ct] : 1.f;
+  float agt = 0.f, abt = 0.f;
   const int64_t step = W == 1 ? (int64_t)nblk * 4 : nblk;
   for (int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x; row < D.rows; row += step) {
-    Raw8 dyr[NV], sr[NV];
+    Raw8 dyr[NV], sr[NV], ir[NV];
     uint32_t byte[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -166,7 +245,7 @@ __global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd
       dyr[i] = raw_load8<DYF>((const char*)D.dy + row * D.lddy * (DYF ? 4 : 2), c, d);
       if (SRC == 0) {
         sr[i].a = u32x4{0, 0, 0, 0};
-        byte[i] = 0;
+        byte[i] = 127;
         if (c < d) {
           const u32x2 w = *reinterpret_cast<const u32x2*>((const uint8_t*)D.q + row * D.ldq + c);
           sr[i].a[0] = w[0]; sr[i].a[1] = w[1];
@@ -176,43 +255,90 @@ __global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd
         sr[i] = raw_load8<SRC == 2>((const char*)D.src + row * D.ldx * (SRC == 2 ? 4 : 2), c, d);
       }
     }
-    const float rs = D.rstd[row], mu = SRC != 0 && D.mean ? D.mean[row] : 0.f;
-    float n[NV][8], h[NV][8], s1 = 0.f, s2 = 0.f;
+    if (D.dx_in) {
+      if (dxf) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = t0 + i * W * 512;
-      float dy[8];
-      raw_values8<DYF>(dyr[i], dy);
-      if (SRC == 0) act8_decode(u32x2{sr[i].a[0], sr[i].a[1]}, byte[i], n[i]);
-      else raw_values8<SRC == 2>(sr[i], n[i]);
+        for (int i = 0; i < NV; ++i) ir[i] = raw_load8<true>((const float*)D.dx_in + row * D.lddx_in, t0 + i * W * 512, d);
+      } else {
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        if (SRC != 0) n[i][r] = (n[i][r] - mu) * rs;
-        if (c + r >= d) n[i][r] = 0.f;               // dy is zero there already
-        h[i][r] = c + r < d ? dy[r] * (D.gamma ? D.gamma[c + r] : 1.f) : 0.f;
-        ag[i][r] = __builtin_fmaf(dy[r], n[i][r], ag[i][r]);
-        ab[i][r] += dy[r];
-        s1 += h[i][r];
-        s2 = __builtin_fmaf(h[i][r], n[i][r], s2);
+        for (int i = 0; i < NV; ++i) ir[i] = raw_load8<false>((const uint16_t*)D.dx_in + row * D.lddx_in, t0 + i * W * 512, d);
       }
     }
-    const float c1 = D.kind == AN_LAYER ? row_sum<W>(s1, red, wave, lane) * inv_d : 0.f;
-    const float c2 = row_sum<W>(s2, red, wave, lane) * inv_d;
+    const float rs = D.rstd[row], mu = SRC != 0 && D.mean ? D.mean[row] : 0.f;
+    float dyt = 0.f, nt = 0.f, it = 0.f;
+    if (T) {
+      dyt = load1<DYF>((const char*)D.dy + row * D.lddy * (DYF ? 4 : 2), ct, d);
+      if (SRC == 0) {
+        if (ct < d) nt = act8_decode1(((const uint8_t*)D.q)[row * D.ldq + ct], ((const uint8_t*)D.scale)[row * D.lds + (ct >> 5)]);
+      } else if (ct < d) {
+        nt = (load1<SRC == 2>((const char*)D.src + row * D.ldx * (SRC == 2 ? 4 : 2), ct, d) - mu) * rs;
+      }
+      if (D.dx_in) it = dxf ? load1<true>((const float*)D.dx_in + row * D.lddx_in, ct, d) : load1<false>((const uint16_t*)D.dx_in + row * D.lddx_in, ct, d);
+    }
+    const auto values = [&](int i, float (&dy)[8], float (&n)[8]) {
+      raw_values8<DYF>(dyr[i], dy);
+      if (SRC == 0) {
+        act8_decode(u32x2{sr[i].a[0], sr[i].a[1]}, byte[i], n);
+      } else {
+        raw_values8<SRC == 2>(sr[i], n);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) n[r] = (n[r] - mu) * rs;
+      }
+      const int c = t0 + i * W * 512;
+      if (c + 8 > d) {                                 // dy is zero there already
+#pragma unroll
+        for (int r = 0; r < 8; ++r) if (c + r >= d) n[r] = 0.f;
+      }
+    };
+    float s1 = 0.f, s2 = 0.f;
+    if (T) {
+      s1 = dyt * gt;
+      s2 = s1 * nt;
+      agt = __builtin_fmaf(dyt, nt, agt);
+      abt += dyt;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float dy[8], n[8];
+      values(i, dy, n);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const float h = dy[r] * gm[i][r];
+        ag[i][r] = __builtin_fmaf(dy[r], n[r], ag[i][r]);
+        ab[i][r] += dy[r];
+        s1 += h;
+        s2 = __builtin_fmaf(h, n[r], s2);
+      }
+    }
+    row_sum2<W>(s1, s2, red, turn, wave, lane);
+    // the values once more from the raw registers (the empty asm keeps the compiler from holding them over the sum: 16 NV registers)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(dyr[i].a), "+v"(sr[i].a));
+    const float c1 = D.kind == AN_LAYER ? s1 * inv_d : 0.f, c2 = s2 * inv_d;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = t0 + i * W * 512;
-      float o[8];
-      if (D.dx_in) {
-        if (D.dx_dtype == VITA_DT_F32) raw_values8<true>(raw_load8<true>((const float*)D.dx_in + row * D.lddx_in, c, d), o);
-        else raw_values8<false>(raw_load8<false>((const uint16_t*)D.dx_in + row * D.lddx_in, c, d), o);
-      }
+      float dy[8], n[8], o[8];
+      values(i, dy, n);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const float t = (h[i][r] - c1 - n[i][r] * c2) * rs;
-        o[r] = c + r < d ? (D.dx_in ? t + o[r] : t) : 0.f;
+      for (int r = 0; r < 8; ++r) o[r] = (dy[r] * gm[i][r] - c1 - n[r] * c2) * rs;
+      if (D.dx_in) {
+        float t[8];
+        if (dxf) raw_values8<true>(ir[i], t); else raw_values8<false>(ir[i], t);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) o[r] += t[r];
       }
-      store8((char*)D.dx + row * D.lddx * (D.dx_dtype == VITA_DT_F32 ? 4 : 2), c, D.lddx, D.dx_dtype == VITA_DT_F32, o);
+      if (c + 8 > d) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) if (c + r >= d) o[r] = 0.f;
+      }
+      store8((char*)D.dx + row * D.lddx * (dxf ? 4 : 2), c, D.lddx, dxf, o);
       if (D.dx_bf16) store8((uint16_t*)D.dx_bf16 + row * D.lddxb, c, D.lddxb, false, o);
+    }
+    if (T) {
+      const float o = ct < d ? (dyt * gt - c1 - nt * c2) * rs + it : 0.f;
+      store1((char*)D.dx + row * D.lddx * (dxf ? 4 : 2), ct, D.lddx, dxf, o);
+      if (D.dx_bf16) store1((uint16_t*)D.dx_bf16 + row * D.lddxb, ct, D.lddxb, false, o);
     }
   }
   if (!D.partial) return;
@@ -228,11 +354,14 @@ __global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd
 #pragma unroll
           for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-              const float a = k ? ab[i][r] : ag[i][r];
-              float* p = &sums[t0 + i * 512 + r];
-              *p = w ? *p + a : a;
+            for (int h = 0; h < 2; ++h) {
+              f32x4* p = reinterpret_cast<f32x4*>(&sums[t0 + i * 512 + 4 * h]);
+              const float (&a)[8] = k ? ab[i] : ag[i];
+              f32x4 t = f32x4{a[4 * h], a[4 * h + 1], a[4 * h + 2], a[4 * h + 3]};
+              if (w) t += *p;
+              *p = t;
             }
+          if (T) sums[ct] = (w ? sums[ct] : 0.f) + (k ? abt : agt);
         }
       }
       __syncthreads();
@@ -249,30 +378,38 @@ __global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd
   }
 }
 
-// column sums of the partial rows: grid (ceil(d / 64), 1 or 2), 16 waves over interleaved rows, fixed order
+// column sums of the partial rows: grid (ceil(d / 32), 1 or 2), 32 rows of threads over interleaved rows, all of a thread's loads in
+// flight at once, fixed order
+#define AN_RED_U ((AN_BWD_MAXBLK + 31) / 32)
 __global__ __launch_bounds__(1024) void addnorm_reduce_kernel(const float* __restrict__ partial, int nblk, int d, float* dgamma,
                                                               float* dbeta, int acc) {
-  __shared__ float red[16][64];
-  const int cx = threadIdx.x & 63, ry = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + cx;
+  __shared__ float red[32][33];
+  const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + cx;
   const float* p = partial + (int64_t)blockIdx.y * nblk * d + c;
-  float a = 0.f;
-  if (c < d)
-    for (int k = ry; k < nblk; k += 16) a += p[(int64_t)k * d];
-  red[ry][cx] = a;
+  float a[AN_RED_U], t = 0.f;
+#pragma unroll
+  for (int u = 0; u < AN_RED_U; ++u) {
+    const int k = ry + 32 * u;
+    a[u] = c < d && k < nblk ? p[(int64_t)k * d] : 0.f;
+  }
+#pragma unroll
+  for (int u = 0; u < AN_RED_U; ++u) t += a[u];
+  red[ry][cx] = t;
   __syncthreads();
   float* o = blockIdx.y ? dbeta : dgamma;
   if (ry == 0 && c < d && o) {
-    float t = 0.f;
+    t = 0.f;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) t += red[w][cx];
+    for (int w = 0; w < 32; ++w) t += red[w][cx];
     o[c] = acc ? o[c] + t : t;
   }
 }
 
 extern "C" int64_t vita_addnorm_bwd_nblk(int64_t rows, int64_t d) {
-  const int64_t n = d <= 1536 ? (rows + 15) / 16 : (rows + 3) / 4;
-  return n < AN_BWD_MAXBLK ? n : AN_BWD_MAXBLK;
+  const int64_t n = d <= 1536 ? (rows + 7) / 8 : (rows + 1) / 2;
+  const int64_t most = d > 1088 && d <= 1536 ? AN_BWD_MAXBLK * 2 / 3 : AN_BWD_MAXBLK;      // as many blocks as are resident: 2 or 3 a CU
+  return n < most ? n : most;
 }
 
 extern "C" int vita_addnorm_bwd(const vita_addnorm_bwd_desc* dp, void* stream) {
@@ -297,26 +434,29 @@ extern "C" int vita_addnorm_bwd(const vita_addnorm_bwd_desc* dp, void* stream) {
     return VITA_ERR_UNSUPPORTED;
   }
   const int nblk = (int)vita_addnorm_bwd_nblk(D.rows, D.d);
+  const int al = ((uintptr_t)D.gamma & 15) == 0;
   const int src = D.q ? 0 : (D.src_dtype == VITA_DT_F32 ? 2 : 1);
-#define AN_LAUNCH(W, NV, SRC, DYF) \
-  hipLaunchKernelGGL((addnorm_bwd_kernel<W, NV, SRC, DYF>), dim3(nblk), dim3(256), 0, (hipStream_t)stream, D, nblk)
-#define AN_TYPES(W, NV)                                                                                                       \
-  do {                                                                                                                        \
-    if (D.dy_dtype == VITA_DT_F32) {                                                                                          \
-      if (src == 0) AN_LAUNCH(W, NV, 0, true); else if (src == 1) AN_LAUNCH(W, NV, 1, true); else AN_LAUNCH(W, NV, 2, true);  \
-    } else {                                                                                                                  \
-      if (src == 0) AN_LAUNCH(W, NV, 0, false); else if (src == 1) AN_LAUNCH(W, NV, 1, false); else AN_LAUNCH(W, NV, 2, false); \
-    }                                                                                                                         \
+#define AN_LAUNCH(W, NV, T, SRC, DYF) \
+  hipLaunchKernelGGL((addnorm_bwd_kernel<W, NV, T, SRC, DYF>), dim3(nblk), dim3(256), 0, (hipStream_t)stream, D, al)
+#define AN_TYPES(W, NV, T)                                                                                                                   \
+  do {                                                                                                                                       \
+    if (D.dy_dtype == VITA_DT_F32) {                                                                                                         \
+      if (src == 0) AN_LAUNCH(W, NV, T, 0, true); else if (src == 1) AN_LAUNCH(W, NV, T, 1, true); else AN_LAUNCH(W, NV, T, 2, true);       \
+    } else {                                                                                                                                 \
+      if (src == 0) AN_LAUNCH(W, NV, T, 0, false); else if (src == 1) AN_LAUNCH(W, NV, T, 1, false); else AN_LAUNCH(W, NV, T, 2, false);    \
+    }                                                                                                                                        \
   } while (0)
-  if (width <= 512) AN_TYPES(1, 1);
-  else if (width <= 1536) AN_TYPES(1, 3);
-  else if (width <= 4096) AN_TYPES(4, 2);
-  else AN_TYPES(4, 4);
+  if (width <= 512) AN_TYPES(1, 1, false);
+  else if (width <= 1024) AN_TYPES(1, 2, false);
+  else if (width <= 1088) AN_TYPES(1, 2, true);
+  else if (width <= 1536) AN_TYPES(1, 3, false);
+  else if (width <= 4096) AN_TYPES(4, 2, false);
+  else AN_TYPES(4, 4, false);
 #undef AN_TYPES
 #undef AN_LAUNCH
   VITA_CHECK_LAUNCH("vita_addnorm_bwd");
   if (D.partial) {
-    hipLaunchKernelGGL(addnorm_reduce_kernel, dim3((unsigned)((D.d + 63) / 64), D.dbeta ? 2 : 1), dim3(1024), 0, (hipStream_t)stream,
+    hipLaunchKernelGGL(addnorm_reduce_kernel, dim3((unsigned)((D.d + 31) / 32), D.dbeta ? 2 : 1), dim3(1024), 0, (hipStream_t)stream,
                        D.partial, nblk, (int)D.d, D.dgamma, D.dbeta, D.accumulate);
     VITA_CHECK_LAUNCH("vita_addnorm_bwd_reduce");
   }
