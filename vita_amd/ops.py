@@ -23,7 +23,9 @@ def _p(t: Optional[torch.Tensor]):
 
 
 def _s():
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream of the current device (torch.cuda.current_stream().cuda_stream without building its Python object: 0.2
+    instead of 2.7 us on the way to every launch)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -360,11 +362,6 @@ class Act8(NamedTuple):
     scale: torch.Tensor
     d: int
 
-    @staticmethod
-    def empty(rows: int, d: int, device) -> "Act8":
-        return Act8(torch.empty(rows, rup(d, 32), dtype=torch.float8_e4m3fn, device=device),
-                    torch.empty(rows, rup(d, 32) // 32, dtype=torch.float8_e8m0fnu, device=device), d)
-
     @property
     def nbytes(self) -> int:
         return self.q.numel() + self.scale.numel()
@@ -383,15 +380,33 @@ _KINDS = {"rms": 0, "layer": 1}
 _PACKS = {None: 0, "normed": 0, "output": 1}
 
 
+_STEP = {torch.bfloat16: 8, torch.float32: 4}         # elements of 16 bytes
+_FLOATS = (torch.bfloat16, torch.float32)
+_BF16 = (torch.bfloat16,)
+
+
 def _on_current_device(t, what):
     if not t.is_cuda:
         raise RuntimeError(f"vita_amd: {what} is on {t.device}; these operators run on an MI355X only (no CPU fallback)")
-    if t.device.index != torch.cuda.current_device():
-        raise RuntimeError(f"vita_amd: {what} is on cuda:{t.device.index} but the current device is cuda:{torch.cuda.current_device()}")
+    if t.get_device() != torch.cuda.current_device():
+        raise RuntimeError(f"vita_amd: {what} is on cuda:{t.get_device()} but the current device is cuda:{torch.cuda.current_device()}")
 
 
-def _mat(t, what, rows=None, d=None, dtypes=(torch.bfloat16, torch.float32)):
+def _mat(t, what, rows=None, d=None, dtypes=_FLOATS):
     """Checks a [rows, d] matrix and returns its row stride in elements."""
+    if isinstance(t, torch.Tensor) and t.dim() == 2 and t.dtype in dtypes and t.is_cuda:
+        n, c = t.shape
+        ld, one = t.stride()
+        step = _STEP[t.dtype]
+        if n == 1:
+            ld = rup(c, step)                          # the only row's stride says nothing
+        if (n and c and (rows is None or n == rows) and (d is None or c == d) and t.get_device() == torch._C._cuda_getDevice()
+                and (one == 1 or c == 1) and ld >= c and ld % step == 0 and t.data_ptr() % 16 == 0):
+            return ld
+    return _refuse_mat(t, what, rows, d, dtypes)
+
+
+def _refuse_mat(t, what, rows, d, dtypes):
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise ValueError(f"vita_amd: {what} must be a 2-D tensor")
     if t.dtype not in dtypes:
@@ -401,28 +416,49 @@ def _mat(t, what, rows=None, d=None, dtypes=(torch.bfloat16, torch.float32)):
     if (rows is not None and t.shape[0] != rows) or (d is not None and t.shape[1] != d):
         raise ValueError(f"vita_amd: {what} has shape {tuple(t.shape)}, expected {(rows, d)}")
     _on_current_device(t, what)
-    step = 16 // t.element_size()
     if t.shape[1] > 1 and t.stride(1) != 1:
         raise ValueError(f"vita_amd: {what} must be contiguous along its last dimension (strides {t.stride()})")
-    ld = t.stride(0) if t.shape[0] > 1 else rup(t.shape[1], step)
-    if t.data_ptr() % 16 or ld % step or ld < t.shape[1]:
-        raise ValueError(f"vita_amd: rows of {what} must start on 16-byte boundaries and must not overlap (strides {t.stride()}, "
-                         f"address % 16 = {t.data_ptr() % 16}); pad the row length to a multiple of {step}")
-    return ld
+    raise ValueError(f"vita_amd: rows of {what} must start on 16-byte boundaries and must not overlap (strides {t.stride()}, "
+                     f"address % 16 = {t.data_ptr() % 16}); pad the row length to a multiple of {_STEP[t.dtype]}")
 
 
 def _vec(t, what, n):
-    """Checks an fp32 vector of n elements (None passes)."""
+    """Checks an fp32 vector of n elements and returns its address (None passes)."""
     if t is None:
         return None
     if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"vita_amd: {what} must be a contiguous float32 tensor of {n} elements, got {t.dtype} {tuple(t.shape)}")
-    _on_current_device(t, what)
+    if not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
+        _on_current_device(t, what)
     return t.data_ptr()
+
+
+def _new_act(rows, d, device):
+    """An empty checkpoint and what the C entries take of it: (Act8, (q pointer, ldq, scale pointer, lds))."""
+    g = (d + 31) // 32
+    q = torch.empty(rows, 32 * g, dtype=torch.float8_e4m3fn, device=device)
+    scale = torch.empty(rows, g, dtype=torch.float8_e8m0fnu, device=device)
+    return Act8(q, scale, d), (q.data_ptr(), 32 * g, scale.data_ptr(), g)
 
 
 def _act(a, what, rows=None):
     """Checks a checkpoint and returns (q pointer, ldq, scale pointer, lds)."""
+    if isinstance(a, Act8) and a.d > 0:
+        q, scale, d = a
+        g = (d + 31) // 32
+        if (q.dtype == torch.float8_e4m3fn and scale.dtype == torch.float8_e8m0fnu and q.dim() == 2 and scale.dim() == 2 and q.is_cuda
+                and scale.is_cuda):
+            n = q.shape[0] if rows is None else rows
+            (ldq, q1), (lds, s1) = q.stride(), scale.stride()
+            if n == 1:
+                ldq, lds = 32 * g, g
+            if (n and tuple(q.shape) == (n, 32 * g) and tuple(scale.shape) == (n, g) and q1 == 1 and (s1 == 1 or g == 1) and ldq >= 32 * g
+                    and lds >= g and ldq % 16 == 0 and q.data_ptr() % 16 == 0 and q.get_device() == scale.get_device() == torch._C._cuda_getDevice()):
+                return q.data_ptr(), ldq, scale.data_ptr(), lds
+    return _refuse_act(a, what, rows)
+
+
+def _refuse_act(a, what, rows):
     if not isinstance(a, Act8):
         raise TypeError(f"vita_amd: {what} must be an Act8")
     if a.d < 1:
@@ -432,29 +468,26 @@ def _act(a, what, rows=None):
         if t.dtype != dt or t.dim() != 2 or t.shape[1] != n or t.shape[0] == 0 or t.shape[0] != (rows if rows is not None else a.q.shape[0]):
             raise ValueError(f"vita_amd: {name} of {what} must be {dt} [{rows if rows is not None else 'rows'}, {n}], got {t.dtype} "
                              f"{tuple(t.shape)}")
-    for t, n, name in ((a.q, 32 * g, "codes"), (a.scale, g, "scales")):
+    for t, name in ((a.q, "codes"), (a.scale, "scales")):
         _on_current_device(t, f"{name} of {what}")
-        if (n > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < n):
-            raise ValueError(f"vita_amd: {name} of {what} have strides {t.stride()}")
-    ldq = a.q.stride(0) if a.q.shape[0] > 1 else 32 * g
-    if ldq % 16 or a.q.data_ptr() % 16:
-        raise ValueError(f"vita_amd: code rows of {what} must start on 16-byte boundaries")
-    return a.q.data_ptr(), ldq, a.scale.data_ptr(), a.scale.stride(0) if a.scale.shape[0] > 1 else g
+    raise ValueError(f"vita_amd: rows of {what} must be contiguous, must not overlap, and code rows must start on 16-byte boundaries (strides "
+                     f"{a.q.stride()}, {a.scale.stride()})")
 
 
 def _ld_out(ld, d, step, what):
-    ld = rup(d, step) if ld is None else int(ld)
+    if ld is None:
+        return (d + step - 1) // step * step
     if ld < d or ld % step:
         raise ValueError(f"vita_amd: {what} = {ld} must be a multiple of {step} and at least {d}")
-    return ld
+    return int(ld)
 
 
 def act8_pack(x) -> Act8:
     """x bf16 | fp32 [rows, d] -> its 8-bit checkpoint."""
     ld = _mat(x, "x")
     rows, d = x.shape
-    a = Act8.empty(rows, d, x.device)
-    check(_lib.lib().vita_act8_pack(x.data_ptr(), _dt(x), ld, rows, d, *_act(a, "the checkpoint"), _s()), "act8_pack")
+    a, ap = _new_act(rows, d, x.device)
+    check(_lib.lib().vita_act8_pack(x.data_ptr(), _dt(x), ld, rows, d, *ap, _s()), "act8_pack")
     return a
 
 
@@ -479,9 +512,8 @@ def gelu_act8_fwd(z, ldg=None):
     rows, d = z.shape
     ldg = _ld_out(ldg, d, 8, "ldg")
     g = torch.empty(rows, ldg, dtype=torch.bfloat16, device=z.device)
-    a = Act8.empty(rows, d, z.device)
-    check(_lib.lib().vita_gelu_act8_fwd(z.data_ptr(), _dt(z), ld, rows, d, g.data_ptr(), ldg, *_act(a, "the checkpoint"), _s()),
-          "gelu_act8_fwd")
+    a, ap = _new_act(rows, d, z.device)
+    check(_lib.lib().vita_gelu_act8_fwd(z.data_ptr(), _dt(z), ld, rows, d, g.data_ptr(), ldg, *ap, _s()), "gelu_act8_fwd")
     return g, a
 
 
@@ -489,7 +521,7 @@ def gelu_act8_bwd(dg, act: Act8, want_g=True, ldo=None):
     """(dg * GELU'(z) bf16 [rows, ldo], GELU(z) bf16 [rows, ldo] or None), z from its checkpoint; zero pads."""
     q = _act(act, "act")
     rows, d = act.q.shape[0], act.d
-    ld = _mat(dg, "dg", rows, d, (torch.bfloat16,))
+    ld = _mat(dg, "dg", rows, d, _BF16)
     ldo = _ld_out(ldo, d, 8, "ldo")
     dz = torch.empty(rows, ldo, dtype=torch.bfloat16, device=dg.device)
     g = torch.empty_like(dz) if want_g else None
@@ -503,7 +535,7 @@ def act8_wgrad(dy, act: Act8, out=None):
     q = _act(act, "act")
     k, n = act.q.shape[0], act.d
     m = dy.shape[-1]
-    ld = _mat(dy, "dy", k, m, (torch.bfloat16,))
+    ld = _mat(dy, "dy", k, m, _BF16)
     if out is not None and out.shape != (m, n):
         raise ValueError(f"vita_amd: out has shape {tuple(out.shape)}, expected {(m, n)}")
     _vec(out, "out", m * n)
@@ -531,32 +563,20 @@ def addnorm_fwd(x, gamma=None, beta=None, residual=None, kind="rms", eps=1e-6, y
     for t in (y_dtype, sum_dtype):
         if t not in (None, torch.bfloat16, torch.float32):
             raise TypeError(f"vita_amd: unsupported dtype {t}")
-    c = AddNormFwdDesc()
-    c.ldx = _mat(x, "x")
+    ldx = _mat(x, "x")
     rows, d = x.shape
     dev = x.device
-    c.x, c.x_dtype, c.rows, c.d = x.data_ptr(), _dt(x), rows, d
-    if residual is not None:
-        c.ldr = _mat(residual, "residual", rows, d)
-        c.res, c.res_dtype = residual.data_ptr(), _dt(residual)
-    c.gamma, c.beta = _vec(gamma, "gamma", d), _vec(beta, "beta", d)
-    c.kind, c.eps, c.pack = _KINDS[kind], eps, _PACKS[pack]
+    ldr = 0 if residual is None else _mat(residual, "residual", rows, d)
+    gp, bp = _vec(gamma, "gamma", d), _vec(beta, "beta", d)
     ld = _ld_out(ldy, d, 8, "ldy")
-    y = s = a = mean = None
-    if y_dtype is not None:
-        y = torch.empty(rows, ld, dtype=y_dtype, device=dev)
-        c.y, c.y_dtype, c.ldy = y.data_ptr(), _dt(y), ld
-    if sum_dtype is not None:
-        s = torch.empty(rows, ld, dtype=sum_dtype, device=dev)
-        c.sum, c.sum_dtype, c.ldsum = s.data_ptr(), _dt(s), ld
-    if pack is not None:
-        a = Act8.empty(rows, d, dev)
-        c.q, c.ldq, c.scale, c.lds = _act(a, "the checkpoint")
+    y = torch.empty(rows, ld, dtype=y_dtype, device=dev) if y_dtype is not None else None
+    s = torch.empty(rows, ld, dtype=sum_dtype, device=dev) if sum_dtype is not None else None
+    a, ap = _new_act(rows, d, dev) if pack is not None else (None, (None, 0, None, 0))
     rstd = torch.empty(rows, dtype=torch.float32, device=dev)
-    if kind == "layer":
-        mean = torch.empty(rows, dtype=torch.float32, device=dev)
-        c.mean = mean.data_ptr()
-    c.rstd = rstd.data_ptr()
+    mean = torch.empty(rows, dtype=torch.float32, device=dev) if kind == "layer" else None
+    c = AddNormFwdDesc(x.data_ptr(), _p(residual), _p(s), gp, bp, _p(y), ap[0], ap[2], _p(mean), rstd.data_ptr(), rows, d,
+                       ldx, ldr, ld, ld, ap[1], ap[3], _KINDS[kind], _PACKS[pack], _dt(x), _dt(residual) if residual is not None else 0,
+                       _dt(s) if s is not None else 0, _dt(y) if y is not None else 0, eps)
     check(_lib.lib().vita_addnorm_fwd(C.byref(c), _s()), "addnorm_fwd")
     return AddNorm(y, s, a, mean, rstd)
 
@@ -570,46 +590,43 @@ def addnorm_bwd(dy, src, rstd, gamma=None, kind="rms", mean=None, dx_in=None, dx
         raise ValueError(f"vita_amd: kind {kind!r}: expected one of {list(_KINDS)}")
     if dx_dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"vita_amd: unsupported dtype {dx_dtype}")
-    c = AddNormBwdDesc()
+    sp = mp = None
+    ldx = src_dt = 0
+    ap = (None, 0, None, 0)
     if isinstance(src, Act8):
-        c.q, c.ldq, c.scale, c.lds = _act(src, "src")
+        ap = _act(src, "src")
         rows, d = src.q.shape[0], src.d
     else:
-        c.ldx = _mat(src, "src")
+        ldx = _mat(src, "src")
         rows, d = src.shape
-        c.src, c.src_dtype = src.data_ptr(), _dt(src)
-        if kind == "layer" and mean is None:
-            raise ValueError("vita_amd: the layer norm's gradient from the sum needs mean")
-        c.mean = _vec(mean, "mean", rows) if kind == "layer" else None
-    dev = rstd.device
-    c.lddy = _mat(dy, "dy", rows, d)
-    c.dy, c.dy_dtype, c.rows, c.d = dy.data_ptr(), _dt(dy), rows, d
-    c.rstd, c.gamma, c.kind = _vec(rstd, "rstd", rows), _vec(gamma, "gamma", d), _KINDS[kind]
+        sp, src_dt = src.data_ptr(), _dt(src)
+        if kind == "layer":
+            if mean is None:
+                raise ValueError("vita_amd: the layer norm's gradient from the sum needs mean")
+            mp = _vec(mean, "mean", rows)
+    lddy = _mat(dy, "dy", rows, d)
+    dev = dy.device
+    rp, gp = _vec(rstd, "rstd", rows), _vec(gamma, "gamma", d)
+    if rp is None:
+        raise ValueError("vita_amd: rstd is missing")
+    ldin = 0 if dx_in is None else _mat(dx_in, "dx_in", rows, d, (dx_dtype,))
     ld = _ld_out(lddx, d, 8, "lddx")
-    dx = torch.empty(rows, ld, dtype=dx_dtype, device=dev)
-    c.dx, c.dx_dtype, c.lddx = dx.data_ptr(), _dt(dx), ld
-    if dx_in is not None:
-        c.lddx_in = _mat(dx_in, "dx_in", rows, d, (dx_dtype,))
-        c.dx_in = dx_in.data_ptr()
-    dxb = None
-    if want_bf16:
-        dxb = torch.empty(rows, ld, dtype=torch.bfloat16, device=dev)
-        c.dx_bf16, c.lddxb = dxb.data_ptr(), ld
     dgamma = dbeta = None
     if acc is not None:
         dg, db = acc
-        c.accumulate = 1
     else:
         want_dbeta = kind == "layer" if want_dbeta is None else want_dbeta
         dg = dgamma = torch.empty(d, dtype=torch.float32, device=dev) if want_dgamma else None
         db = dbeta = torch.empty(d, dtype=torch.float32, device=dev) if want_dbeta else None
     if kind == "rms" and db is not None:
         raise ValueError("vita_amd: the rms norm has no beta")
-    c.dgamma, c.dbeta = _vec(dg, "dgamma", d), _vec(db, "dbeta", d)
+    dgp, dbp = _vec(dg, "dgamma", d), _vec(db, "dbeta", d)
+    dx = torch.empty(rows, ld, dtype=dx_dtype, device=dev)
+    dxb = torch.empty(rows, ld, dtype=torch.bfloat16, device=dev) if want_bf16 else None
     partial = None
     if dg is not None or db is not None:
-        nblk = _lib.lib().vita_addnorm_bwd_nblk(rows, d)
-        partial = torch.empty(2 * nblk * d, dtype=torch.float32, device=dev)
-        c.partial = partial.data_ptr()
+        partial = torch.empty(2 * _lib.lib().vita_addnorm_bwd_nblk(rows, d) * d, dtype=torch.float32, device=dev)
+    c = AddNormBwdDesc(dy.data_ptr(), sp, ap[0], ap[2], mp, rp, gp, _p(dx_in), dx.data_ptr(), _p(dxb), dgp, dbp, _p(partial), rows, d,
+                       lddy, ldx, ap[1], ap[3], ldin, ld, ld, _KINDS[kind], int(acc is not None), _dt(dy), src_dt, _dt(dx))
     check(_lib.lib().vita_addnorm_bwd(C.byref(c), _s()), "addnorm_bwd")
     return (dx, dxb) if want_bf16 else dx, dgamma, dbeta
