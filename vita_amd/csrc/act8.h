@@ -116,8 +116,11 @@ __device__ __forceinline__ void raw_values8(const Raw8& w, float (&v)[8]) {
     else v[r] = __builtin_bit_cast(float, (r & 1) ? (w.a[r >> 1] & 0xffff0000u) : (w.a[r >> 1] << 16));
   }
 }
-__device__ __forceinline__ u32x4 pack_bf16x8(const float (&v)[8]) {
-  return u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+__device__ __forceinline__ u32x4 pack_bf16x8(const float (&v)[8]) {      // four v_cvt_pk_bf16_f32
+  bf16x8 o;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) o[r] = (__bf16)v[r];
+  return __builtin_bit_cast(u32x4, o);
 }
 // 8 neighbouring floats of a vector of d (gamma, beta), `fill` behind its end and for NULL; al: 16-byte aligned
 __device__ __forceinline__ void vec_load8(const float* p, int c, int d, bool al, float fill, float (&v)[8]) {

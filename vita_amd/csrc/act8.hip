@@ -1,8 +1,20 @@
 // 8-bit activation checkpoints (act8.h: format): packing, restoring, and GELU with its checkpoint in one pass.
 //
 // All of these move bytes: a lane takes 8 neighbouring columns, the chunks of a matrix are numbered row by row and dealt to the
-// threads in order, so that narrow, wide and odd rows fill the chip alike.
+// threads in order, so that narrow, wide and odd rows fill the chip alike.  One chunk to a thread: two or four with their loads
+// together are no faster (GELU backward 46082 x 4100: 250, 264, 284 us).  Measured (MI355X, kernels alone; a copy reaches 5 TB/s):
+//   pack 13826 x 1025 fp32 13 us (5.4 TB/s); restore it with gamma and beta 12 us (one load for each element of gamma: 55 us)
+//   GELU forward 13826 x 4100 60 us (4.8 TB/s), 3776 x 4100 18 us; backward 46082 x 4100 250 us (5.3 TB/s), 3776 x 4100 22 us (about 36
+//   issue slots an element, 8 of them exp and rcp: two thirds of the time at this size)
 #include "act8.h"
+
+// the values of 8 neighbouring codes; zeros behind the row's end
+__device__ __forceinline__ void codes_load8(const uint8_t* q, const uint8_t* scale, int c, int d, float (&v)[8]) {
+  u32x2 w = {0, 0};
+  uint32_t byte = 127;
+  if (c < d) { w = *reinterpret_cast<const u32x2*>(q + c); byte = scale[c >> 5]; }
+  act8_decode(w, byte, v);
+}
 
 struct ChunkMap {      // chunk number -> (row, column) for rows of nc chunks
   int64_t rows;
@@ -10,26 +22,22 @@ struct ChunkMap {      // chunk number -> (row, column) for rows of nc chunks
 };
 
 #define A8_THREADS 256
-#define A8_UNROLL 2
 
+// f(row, c) for this thread's chunk
 template <typename F>
-__device__ __forceinline__ void for_chunks(const ChunkMap M, F f) {
-  const int64_t base = (int64_t)blockIdx.x * (A8_THREADS * A8_UNROLL);
+__device__ __forceinline__ void for_chunk(const ChunkMap M, F f) {
+  const int64_t base = (int64_t)blockIdx.x * A8_THREADS;
   const int64_t row0 = base / M.nc;
-  const uint32_t col0 = (uint32_t)(base - row0 * M.nc);
-#pragma unroll
-  for (int u = 0; u < A8_UNROLL; ++u) {
-    const uint32_t t = col0 + u * A8_THREADS + threadIdx.x;
-    const uint32_t dr = t / M.nc;
-    const int64_t row = row0 + dr;
-    if (row < M.rows) f(row, (int)(t - dr * M.nc) * 8);      // M.nc % 4 == 0: a quad never straddles two rows
-  }
+  const uint32_t t = (uint32_t)(base - row0 * M.nc) + threadIdx.x;      // < nc + A8_THREADS
+  const uint32_t dr = M.nc >= A8_THREADS ? (t >= M.nc ? 1u : 0u) : t / M.nc;
+  const int64_t row = row0 + dr;
+  if (row < M.rows) f(row, (int)(t - dr * M.nc) * 8);                    // M.nc % 4 == 0: a quad never straddles two rows
 }
 static bool chunk_grid(int64_t rows, int64_t cols, ChunkMap& M, dim3& grid) {
   if (rows > ((int64_t)1 << 40)) return false;
   M.rows = rows;
   M.nc = (uint32_t)((cols + ACT8_GROUP - 1) / ACT8_GROUP * (ACT8_GROUP / 8));
-  const int64_t blocks = (rows * M.nc + A8_THREADS * A8_UNROLL - 1) / (A8_THREADS * A8_UNROLL);
+  const int64_t blocks = (rows * M.nc + A8_THREADS - 1) / A8_THREADS;
   grid = dim3((unsigned)blocks);
   return blocks < (int64_t)0x7fffffff;
 }
@@ -38,7 +46,7 @@ template <bool F32>
 __global__ __launch_bounds__(A8_THREADS) void act8_pack_kernel(const void* __restrict__ x, int64_t ldx, ChunkMap M, int d,
                                                                uint8_t* __restrict__ q, int64_t ldq, uint8_t* __restrict__ scale,
                                                                int64_t lds) {
-  for_chunks(M, [&](int64_t row, int c) {
+  for_chunk(M, [&](int64_t row, int c) {
     float v[8];
     raw_values8<F32>(raw_load8<F32>((const char*)x + row * ldx * (F32 ? 4 : 2), c, d), v);
     uint32_t byte;
@@ -70,10 +78,10 @@ __global__ __launch_bounds__(A8_THREADS) void act8_unpack_kernel(const uint8_t* 
                                                                  const uint8_t* __restrict__ scale, int64_t lds, ChunkMap M, int d,
                                                                  const float* __restrict__ gamma, const float* __restrict__ beta, int al,
                                                                  void* __restrict__ y, int64_t ldy, int y_f32) {
-  for_chunks(M, [&](int64_t row, int c) {
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for_chunk(M, [&](int64_t row, int c) {
+    float v[8];
+    codes_load8(q + row * ldq, scale + row * lds, c, d, v);
     if (c < d) {
-      act8_decode(*reinterpret_cast<const u32x2*>(q + row * ldq + c), scale[row * lds + (c >> 5)], v);
       if (gamma) {
         float g[8], b[8];
         vec_load8(gamma, c, d, al, 0.f, g);
@@ -109,7 +117,7 @@ template <bool F32>
 __global__ __launch_bounds__(A8_THREADS) void gelu_act8_fwd_kernel(const void* __restrict__ z, int64_t ldz, ChunkMap M, int d,
                                                                    uint16_t* __restrict__ g, int64_t ldg, uint8_t* __restrict__ q,
                                                                    int64_t ldq, uint8_t* __restrict__ scale, int64_t lds) {
-  for_chunks(M, [&](int64_t row, int c) {
+  for_chunk(M, [&](int64_t row, int c) {
     float v[8];
     raw_values8<F32>(raw_load8<F32>((const char*)z + row * ldz * (F32 ? 4 : 2), c, d), v);
     uint32_t byte;
@@ -147,16 +155,19 @@ __global__ __launch_bounds__(A8_THREADS) void gelu_act8_bwd_kernel(const uint16_
                                                                    int64_t ldq, const uint8_t* __restrict__ scale, int64_t lds,
                                                                    ChunkMap M, int d, uint16_t* dz, int64_t lddz,
                                                                    uint16_t* __restrict__ g, int64_t ldg) {
-  for_chunks(M, [&](int64_t row, int c) {
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, t[8], p[8];
+  for_chunk(M, [&](int64_t row, int c) {
+    float v[8], t[8], p[8];
     raw_values8<false>(raw_load8<false>(dg + row * lddg, c, d), t);
-    if (c < d) act8_decode(*reinterpret_cast<const u32x2*>(q + row * ldq + c), scale[row * lds + (c >> 5)], v);
+    codes_load8(q + row * ldq, scale + row * lds, c, d, v);
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       float der;
       gelu_erf_both(v[r], p[r], der);
       t[r] *= der;
-      if (c + r >= d) t[r] = p[r] = 0.f;
+    }
+    if (c + 8 > d) {                        // codes behind d are whatever the caller's buffer holds
+#pragma unroll
+      for (int r = 0; r < 8; ++r) if (c + r >= d) t[r] = p[r] = 0.f;
     }
     store8(dz + row * lddz, c, lddz, false, t);
     if (g) store8(g + row * ldg, c, ldg, false, p);
