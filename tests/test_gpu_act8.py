@@ -227,7 +227,8 @@ def _check_norm(ops, x, res, gamma, beta, kind, eps, y_dtype, sum_dtype, pack, l
 
 
 @pytest.mark.parametrize("kind", ["rms", "layer"])
-@pytest.mark.parametrize("rows,d", SHAPES)
+@pytest.mark.parametrize("rows,d", SHAPES + [(1500, 1025), (1100, 600), (1030, 1000), (1030, 1060), (1030, 1100), (1030, 1500), (1030, 2000),
+                                             (20000, 40)])
 def test_addnorm_fwd_shapes(ops, rows, d, kind):
     x, res, gamma, beta = _norm_case(rows, d, BF16, F32, kind, rows + d)
     _check_norm(ops, x, res, gamma, beta, kind, 1e-5, BF16, F32, "normed", ldy=(d + 63) // 64 * 64 if d < 8100 else None)
@@ -259,6 +260,17 @@ def test_addnorm_fwd_hard_rows(ops):
         assert torch.equal(a.y[:6], clean.y) and torch.equal(a.act.q[:6].view(torch.uint8), clean.act.q.view(torch.uint8))
         assert torch.isnan(a.y[6, :d]).all() and torch.isnan(R.values(a.act)[6]).all()
         assert torch.isnan(a.y[7, 5]) and torch.isfinite(a.y[8, :d]).all()
+        zero_pads(a.y, d)                                # also in the rows that are NaN
+        assert torch.count_nonzero(a.act.q.view(torch.uint8)[:, d:]) == 0
+    wide = torch.randn(3, 1032, device="cuda")[:, :1025]
+    wide[1, 1024] = float("nan")
+    many = torch.zeros(2100, 1032, device="cuda")[:, :1025]      # more rows: another kernel
+    many.copy_(wide.repeat(700, 1))
+    for rows in (wide, many):
+        a = ops.addnorm_fwd(rows, kind="layer", eps=1e-5, y_dtype=BF16, pack="normed", ldy=1088)
+        zero_pads(a.y, 1025)
+        assert torch.count_nonzero(a.act.q.view(torch.uint8)[:, 1025:]) == 0
+        assert torch.isnan(a.y[1, :1025]).all() and torch.isfinite(a.y[0, :1025]).all() and torch.isfinite(a.y[2, :1025]).all()
 
 
 # ------------------------------------------------------------------------------------------------ norms, backward
@@ -305,7 +317,7 @@ def _check_bwd(ops, rows, d, kind, src_kind, dyt, dxt, with_in, seed, gamma=True
 
 @pytest.mark.parametrize("kind", ["rms", "layer"])
 @pytest.mark.parametrize("src", ["act8", "f32"])
-@pytest.mark.parametrize("rows,d", SHAPES + [(4000, 129)])
+@pytest.mark.parametrize("rows,d", SHAPES + [(4000, 129), (3000, 1025), (500, 600), (300, 1000), (300, 1060), (300, 1100), (300, 1500), (300, 2000)])
 def test_addnorm_bwd_shapes(ops, rows, d, src, kind):
     _check_bwd(ops, rows, d, kind, src, BF16, F32, True, rows + d)
 

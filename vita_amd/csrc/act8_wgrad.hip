@@ -313,7 +313,8 @@ static Wgrad8Plan w8_plan(int64_t m, int64_t n, int64_t k) {
     const int nf = cand[c];
     const int64_t tiles = tm * ((n + nf * 16 - 1) / (nf * 16));
     const int64_t whole = tiles / W8_WGS * W8_WGS, left = tiles - whole;
-    for (int64_t cut = 1; cut <= W8_WGS && (cut == 1 || kt / cut >= 4); ++cut) {
+    const int64_t most = left ? (W8_WGS + left - 1) / left : 1;      // more parts than that leave tiles for the line
+    for (int64_t cut = 1; cut <= most && (cut == 1 || kt / cut >= 4); cut = cut < 8 || cut + 1 >= most - 1 ? cut + 1 : cut * 2 < most - 1 ? cut * 2 : most - 1) {
       int64_t ct = W8_WGS / cut; if (ct > left) ct = left;
       const int64_t line = (left - ct) * kt;
       int64_t piece = (line + W8_WGS - 1) / W8_WGS;

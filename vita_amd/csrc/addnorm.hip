@@ -135,7 +135,11 @@ __global__ __launch_bounds__(256) void addnorm_fwd_kernel(const vita_addnorm_fwd
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         v[i][r] = __builtin_fmaf(v[i][r], rs, v[i][r] * rl);
-        y[r] = __builtin_fmaf(v[i][r], gm[i][r], bt[i][r]);        // 0 * 1 + 0 behind the row's end
+        y[r] = __builtin_fmaf(v[i][r], gm[i][r], bt[i][r]);
+      }
+      if (c + 8 > d) {                         // zeros behind the row's end, also in a row whose rstd is NaN
+#pragma unroll
+        for (int r = 0; r < 8; ++r) if (c + r >= d) v[i][r] = y[r] = 0.f;
       }
       if (D.q) {
         uint32_t byte;
@@ -148,8 +152,8 @@ __global__ __launch_bounds__(256) void addnorm_fwd_kernel(const vita_addnorm_fwd
       if (D.y) store8((char*)D.y + row * D.ldy * (D.y_dtype == VITA_DT_F32 ? 4 : 2), c, D.ldy, D.y_dtype == VITA_DT_F32, y);
     }
     if (T) {
-      vt = __builtin_fmaf(vt, rs, vt * rl);
-      const float y = __builtin_fmaf(vt, gt, btt);
+      vt = ct < d ? __builtin_fmaf(vt, rs, vt * rl) : 0.f;
+      const float y = ct < d ? __builtin_fmaf(vt, gt, btt) : 0.f;
       if (D.q) {
         uint32_t byte;
         const uint8_t w = act8_encode1(D.pack == VITA_PACK_OUTPUT ? y : vt, byte);

@@ -207,6 +207,8 @@ class Masker:
 
 # ----------------------------------------------------------------------------- encoder
 class ImagingMaskedEncoder(nn.Module):
+    saved_bits = 16          # modules pickled before the option existed
+
     def __init__(self, *args, **kwargs):
         super().__init__()
         self.enc_embed_dim = kwargs.get("enc_embed_dim")
@@ -224,7 +226,7 @@ class ImagingMaskedEncoder(nn.Module):
         self.use_both_axes = kwargs.get("use_both_axes")
         self.patch_p_num = np.prod(kwargs.get("patch_size")) * self.patch_in_channels
         self.grad_checkpointing = kwargs.get("grad_checkpointing", False)
-        self.saved_bits = kwargs.get("saved_bits", 16)          # 8: activations kept for the backward pass in 8 bits
+        self.saved_bits = kwargs.get("saved_bits") or 16        # 8: activations kept for the backward pass in 8 bits
         norm_layer = kwargs.get("norm_layer") or nn.LayerNorm
         self.pixel_unshuffle_scale = kwargs.get("pixel_unshuffle_scale")
         self.patch_embed = PatchEmbed(self.img_shape, in_channels=self.patch_in_channels,
@@ -306,6 +308,8 @@ class ImagingMaskedEncoder(nn.Module):
 
 # ----------------------------------------------------------------------------- decoder (adjacent)
 class ViTDecoder(nn.Module):
+    saved_bits = 16          # modules pickled before the option existed
+
     def __init__(self, dim, num_heads, depth, mlp_ratio, norm_layer=nn.LayerNorm, grad_checkpointing: bool = False, saved_bits: int = 16):
         super().__init__()
         self.saved_bits = saved_bits
@@ -328,6 +332,8 @@ class ViTDecoder(nn.Module):
 
 
 class ImagingMaskedDecoder(nn.Module):
+    saved_bits = 16          # modules pickled before the option existed
+
     def __init__(self, *args, **kwargs):
         super().__init__()
         self.grid_size = kwargs.get("grid_size")
@@ -341,8 +347,8 @@ class ImagingMaskedDecoder(nn.Module):
                                           requires_grad=False)
         self.decoder = ViTDecoder(dim=kwargs.get("dec_embed_dim"), num_heads=kwargs.get("dec_num_heads"),
                                   depth=kwargs.get("dec_depth"), mlp_ratio=kwargs.get("mlp_ratio"),
-                                  norm_layer=kwargs.get("norm_layer") or nn.LayerNorm, saved_bits=kwargs.get("saved_bits", 16))
-        self.saved_bits = kwargs.get("saved_bits", 16)
+                                  norm_layer=kwargs.get("norm_layer") or nn.LayerNorm, saved_bits=kwargs.get("saved_bits") or 16)
+        self.saved_bits = kwargs.get("saved_bits") or 16
         self.recon_head = nn.Linear(in_features=kwargs.get("dec_embed_dim"), out_features=kwargs.get("head_out_dim"))
         self.mask_token = nn.Parameter(torch.zeros(1, 1, self.dec_embed_dim), requires_grad=True)
         self.head_out_dim = int(kwargs.get("head_out_dim"))
@@ -395,10 +401,12 @@ class TabularViT(nn.Module):
     output [B, 1 + n_features, D].  The 117 per-feature tokenizers are evaluated as two batched torch ops
     (they are a few KB of parameters); the transformer blocks and the LayerNorm run in libvita_hip.so."""
 
+    saved_bits = 16
+
     def __init__(self, args, all_feature_names: dict, **kwargs) -> None:
         super().__init__()
         self.grad_checkpointing = args.grad_checkpointing
-        self.saved_bits = getattr(args, "saved_bits", 16)       # 8: activations kept for the backward pass in 8 bits
+        self.saved_bits = getattr(args, "saved_bits", None) or 16   # 8: activations kept for the backward pass in 8 bits
         self.embedding_dim = args.embedding_dim
         self.all_feature_names = all_feature_names
         self.num_numerical = len(all_feature_names["numerical"])

@@ -661,6 +661,8 @@ class Block(nn.Module):
       norm_layer=nn.RMSNorm  root-mean-square norms
       saved_bits=8           activations kept for the backward pass in 8 bits (_BlockActFn); 16 keeps them as computed"""
 
+    saved_bits = 16          # modules pickled before the option existed
+
     def __init__(self, dim, num_heads, mlp_ratio=4., qkv_bias=False, drop=0., attn_drop=0., init_values=None,
                  drop_path=0., act_layer=nn.GELU, norm_layer=nn.LayerNorm, saved_bits=16):
         super().__init__()
