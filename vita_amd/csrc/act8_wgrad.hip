@@ -3,10 +3,10 @@
 // value = code * 2^e is exact in bf16 (act8.h), so the codes are turned into bf16 on their way into LDS and the products run on
 // v_mfma_f32_16x16x32_bf16 with no rounding beyond fp32 accumulation: nothing of the restored matrix ever reaches HBM.
 //
-//   * 256 x (16 NF) x 64 tiles, 8 waves (4 x 2), the pipeline of gemm256.hip: dy goes HBM -> LDS by LDS-DMA, fragments are read
-//     with ds_read_b64_tr_b16 under the MFMAs, one barrier per K-tile.  A code tile goes through registers: 16
-//     codes and their scale byte per load, fetched a whole K-tile before they are needed; behind the barrier that frees their stage
-//     they are converted and written (16 conversions, 4 ds_write_b128 per thread and K-tile) under the first matrix instructions.
+//   * 256 x (16 NF) x 64 tiles, 8 waves (4 x 2), LDS images and fragments of gemm256.hip: dy goes HBM -> LDS by LDS-DMA, fragments are
+//     read with ds_read_b64_tr_b16.  A code tile goes through registers: 16 codes and their scale byte per load, fetched a whole
+//     K-tile before they are needed, converted and written (16 conversions, 4 ds_write_b128 per thread and K-tile) between the
+//     matrix instructions.  The two waves of a SIMD take turns at the matrix pipe (schedule at the loop).
 //   * a weight matrix gives few tiles (1025 x 4100: 85) and a token count long sums, so tiles are cut along the tokens (w8_plan):
 //     whole rounds of 256 tiles stay whole, of the others as many as fit are cut into `cut` equal parts, one per workgroup, and
 //     what is left over is dealt out in short pieces behind those.  Equal cuts keep the workgroups of an XCD (blockIdx % 8) on the
@@ -16,13 +16,14 @@
 //   * a part of a tile goes to the workspace as fp32; a second kernel adds a tile's parts in their order.  One writer per
 //     element, no atomics: the same bits on every call.
 //
-// Measured (MI355X): 3776 tokens, 1025 x 4100: 44 + 15 us (join), 720 TFLOP/s without the join; 13826 tokens, 1025 x 3075: 114 + 15 us;
-// the bf16 kernel of gemm256.hip with atomics takes 85 and 131 us for the same shapes, without the pass that restores its operand.  A
-// K-tile takes 1.48 us at 208 columns: 0.87 us of matrix instructions and barriers, the rest LDS reads (+0.18) and the operands' way
-// into LDS (+0.4; no better with the loads' data in L2, without the waits for dy, with four waves of twice the rows (124 us), or with
-// the conversions later in the K-tile (121 us) or staggered between the two halves of the workgroup (137 us)).
+// Measured (MI355X): 3776 tokens, 1025 x 4100: 42 + 15 us (join), 750 TFLOP/s without the join; 13826 tokens, 1025 x 3075: 109 + 15 us,
+// 800 TFLOP/s; the bf16 kernel of gemm256.hip with atomics takes 85 and 131 us for the same shapes, without the pass that restores its
+// operand.  Bound by what one wave after another can issue: without the conversions 98 us of the 109 are left, without the DMA of dy
+// 96, without either 85 (matrix instructions, fragment reads, barriers); without the loads of the codes 109.  With all waves in step and
+// the conversions in one piece behind the barrier the two shapes take 43 and 114 to 122 us; with four waves of twice the rows 124.
 #include "act8.h"
 #include "gemm256.h"
+#include <type_traits>
 
 #define W8_WGS 256               // workgroups of a full round: one per CU
 
@@ -54,9 +55,11 @@ __device__ __forceinline__ int64_t w8_piece_slot(const Wgrad8Params& P, int piec
 __device__ __forceinline__ int w8_cut_begin(const Wgrad8Params& P, int part) { return (int)((int64_t)P.kt * part / P.cut); }
 
 __device__ __forceinline__ uint64_t w8_uniform(uint64_t v) { return ((uint64_t)g2_sgpr((uint32_t)(v >> 32)) << 32) | g2_sgpr((uint32_t)v); }
-// descriptor of the bytes [adv, bytes) behind base, all in scalar registers
+// descriptor of the bytes [adv, bytes) behind base; operands uniform and below 2^31 (the host checks them).  The maximum is a signed one
+// because that stays on the scalar unit: a compare and select went to vector registers, and the loads into loops over lanes.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t w8_rsrc(uint64_t base, uint32_t adv, uint32_t bytes) {
-  return g2_rsrc((const void*)(base + adv), g2_sgpr(adv < bytes ? bytes - adv : 0u));
+  const int rem = (int)bytes - (int)adv;
+  return g2_rsrc((const void*)(base + adv), (uint32_t)(rem > 0 ? rem : 0));
 }
 
 template <int NF>
@@ -125,115 +128,144 @@ __global__ __launch_bounds__(G2_THREADS, 2) void act8_wgrad_kernel(const Wgrad8P
 
     LoaderA la;
     la.init(P.dy + k0 * P.lddy, m0, P.m, krows, P.lddy, wave, lane);
-    G2Frags<1, 4> fa;
-    G2Frags<1, NFW> fb;
-    fa.init(wm * 4, 0, lane);
-    fb.init(wn * NFW, BOFF, lane);
-
     // bounds-checked loads: tokens past the part and columns past the codes arrive as zeros
     const uint32_t col_on = bcol < NF && n0 + bcol * 16 < ncodes;
-    const uint32_t qoff = col_on ? (uint32_t)(brow * P.ldq) + bcol * 16 : G2_OOB;
-    const uint32_t soff = col_on ? (uint32_t)(brow * P.lds) + (((uint32_t)(n0 & 31) + bcol * 16) >> 5) : G2_OOB;
+    uint32_t qoff[2], soff[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      qoff[i] = col_on ? (uint32_t)((brow + 32 * i) * P.ldq) + bcol * 16 : G2_OOB;
+      soff[i] = col_on ? (uint32_t)((brow + 32 * i) * P.lds) + (((uint32_t)(n0 & 31) + bcol * 16) >> 5) : G2_OOB;
+    }
+    const uint64_t abase = w8_uniform((uint64_t)(P.dy + k0 * P.lddy + m0));
     const uint64_t qbase = w8_uniform((uint64_t)(P.q + k0 * P.ldq + n0)), sbase = w8_uniform((uint64_t)(P.scale + k0 * P.lds + (n0 >> 5)));
     const uint32_t qbytes = g2_sgpr((uint32_t)((krows - 1) * P.ldq + (ncodes - n0)));
     const uint32_t sbytes = g2_sgpr((uint32_t)((krows - 1) * P.lds + ((ncodes >> 5) - (n0 >> 5))));
-    auto b_load = [&](int t, int i, u32x4& q, uint32_t& sc) {
-      const uint32_t r = (uint32_t)t * G2_BK + 32 * i;
-      const uint32_t qa = g2_sgpr(r * (uint32_t)P.ldq), sa = g2_sgpr(r * (uint32_t)P.lds);
-      q = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(w8_rsrc(qbase, qa, qbytes), qoff, 0, 0));
-      sc = __builtin_amdgcn_raw_buffer_load_b8(w8_rsrc(sbase, sa, sbytes), soff, 0, 0);
-    };
-    // 16 codes -> 16 bf16 -> LDS.  The writes are inline asm: the compiler would wait for every LDS-DMA in flight before a write of
-    // its own.  Their results are waited for with the fragment reads (lgkmcnt(0) before the barrier).
-    auto b_write = [&](int stage, int i, const u32x4& q, uint32_t sc) {
-      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-      const float s = act8_scale(sc);
-      u32x4 o[2];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        o[j >> 1][2 * (j & 1)] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q[j], s, false));
-        o[j >> 1][2 * (j & 1) + 1] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q[j], s, true));
-      }
-      const uint32_t at = boff + stage * STAGE + i * 16384;
-      asm volatile("ds_write_b128 %0, %1" :: "v"(at), "v"(o[0]) : "memory");
-      asm volatile("ds_write_b128 %0, %1 offset:16" :: "v"(at), "v"(o[1]) : "memory");
-    };
+    const uint32_t qstep = g2_sgpr((uint32_t)(G2_BK * P.ldq)), sstep = g2_sgpr((uint32_t)(G2_BK * P.lds));
+    auto a_rsrc = [&](int t) { return w8_rsrc(abase, (uint32_t)t * la.kstep, la.bytes); };
+    auto q_rsrc = [&](int t) { return w8_rsrc(qbase, (uint32_t)t * qstep, qbytes); };
+    auto s_rsrc = [&](int t) { return w8_rsrc(sbase, (uint32_t)t * sstep, sbytes); };
     u32x4 qv[2];
     uint32_t sv[2];
+    auto b_load = [&](__amdgpu_buffer_rsrc_t rq, __amdgpu_buffer_rsrc_t rs, int i) {
+      qv[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rq, qoff[i], 0, 0));
+      sv[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, soff[i], 0, 0);
+    };
+    // 16 codes -> 16 bf16 -> LDS in six steps: four codes each, then the two halves written.  The writes are inline asm: the compiler
+    // would wait for every LDS-DMA in flight before a write of its own.  They are waited for with the fragment reads (lgkmcnt(0)).
+    u32x4 bo[2];
+    auto b_step = [&](int stage, int i, int step) {
+      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+      if (step < 4) {
+        const float sc = act8_scale(sv[i]);
+        bo[step >> 1][2 * (step & 1)] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)qv[i][step], sc, false));
+        bo[step >> 1][2 * (step & 1) + 1] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)qv[i][step], sc, true));
+      } else {
+        const uint32_t at = boff + stage * STAGE + i * 16384;
+        if (step == 4) asm volatile("ds_write_b128 %0, %1" :: "v"(at), "v"(bo[0]) : "memory");
+        else asm volatile("ds_write_b128 %0, %1 offset:16" :: "v"(at), "v"(bo[1]) : "memory");
+      }
+    };
 
     f32x4 acc[4][NFW];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < NFW; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    bf16x8 a0[4], b0[NFW], a1[4], b1[NFW];
-    // operands swapped: a lane ends up with 4 neighbouring columns of one row
-#define W8_MFMA_GROUP(J, AF, BF)                                                                       \
-  if (NF % 2 == 0 || (J) < NFW - 1 || wn == 0) {                                                       \
-    _Pragma("unroll") for (int i = 0; i < 4; ++i)                                                      \
-      acc[i][J] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(BF[J], AF[i], acc[i][J], 0, 0, 0);           \
-  }
-#define W8_READ_B(KS, BF, LO, HI) fb.template read_range<KS, true, LO, HI, NFW>(smem, BF)
-#define W8_READ_A(KS, AF) fa.template read_range<KS, true, 0, 4, 4>(smem, AF)
-    // every fragment read issued so far has landed (the compiler cannot see those reads)
-#define W8_WAIT_FRAGS() do { __builtin_amdgcn_s_waitcnt(0xc07f); __builtin_amdgcn_sched_barrier(0); } while (0)
-#define W8_PHASE1()                                                  \
-  W8_WAIT_FRAGS();                                                   \
-  _Pragma("unroll") for (int j = 0; j < NFW; ++j) {                  \
-    if (j == 0) { W8_READ_A(1, a1); W8_READ_B(1, b1, 0, 1); }        \
-    if (j == 1) { W8_READ_B(1, b1, 1, 4); }                          \
-    if (j == 2) { W8_READ_B(1, b1, 4, NFW); }                        \
-    W8_MFMA_GROUP(j, a0, b0);                                        \
-    __builtin_amdgcn_sched_barrier(0);                               \
-  }
-    // K-tiles 0 and 1 in one memory latency (one past the end: dy arrives as zeros, the codes are taken as zeros)
+
+    // K-tile 0, and the codes of K-tile 1 on their way (past the end: dy arrives as zeros, the codes are taken as zeros)
     {
-      const __amdgpu_buffer_rsrc_t ra = la.rsrc(0), rb = la.rsrc(1);
+      const __amdgpu_buffer_rsrc_t ra = a_rsrc(0), rq = q_rsrc(0), rs = s_rsrc(0), rq1 = q_rsrc(1), rs1 = s_rsrc(1);
 #pragma unroll
       for (int i = 0; i < PA; ++i) la.issue(ra, true, i, smem, wave);
+      b_load(rq, rs, 0); b_load(rq, rs, 1);
+      __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this wave's pieces of dy are in LDS
 #pragma unroll
-      for (int i = 0; i < PA; ++i) la.issue(rb, true, i, smem + STAGE, wave);
-      u32x4 q1[2];
-      uint32_t s1[2];
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) { b_load(0, i, qv[i], sv[i]); b_load(1, i, q1[i], s1[i]); }
-      __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this wave's pieces of both K-tiles of dy are in LDS
-#pragma unroll
-      for (int i = 0; i < 2; ++i) { b_write(0, i, qv[i], sv[i]); b_write(1, i, q1[i], s1[i]); b_load(2, i, qv[i], sv[i]); }
+        for (int k = 0; k < 6; ++k) b_step(0, i, k);
+        b_load(rq1, rs1, i);
+      }
     }
     __builtin_amdgcn_s_waitcnt(0xc07f);        // lgkmcnt(0): the codes too
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    W8_READ_A(0, a0); W8_READ_B(0, b0, 0, NFW);
-    for (int t = 0; t + 1 < nkt; ++t) {
-      W8_PHASE1();
-      // K-tile t+1 is complete in LDS for every wave, and every wave has read K-tile t: its stage is free for K-tile t+2
-      g2_sync_all();
-      fa.toggle((t & 1) ? -STAGE : STAGE); fb.toggle((t & 1) ? -STAGE : STAGE);
-      const __amdgpu_buffer_rsrc_t ra = la.rsrc(t + 2);
-      char* st = smem + (t & 1) * STAGE;
+
+    // The two waves of a SIMD take turns.  Time goes in slots between barriers; in a K-tile a wave has four: it reads the fragments of
+    // the first half (M0), multiplies them (C0), reads (M1) and multiplies (C1) the second half, and the second half of the workgroup
+    // does the same one slot later, so that the matrix pipe of a SIMD always has one wave that feeds it.  A wave issues in order: what
+    // else it does in C0 and C1 stands between its matrix instructions, two or three instructions at a time.  With slots counted from
+    // the first group's M0 of K-tile t, its own slots are 0 1 2 3, the second group's 1 2 3 4:
+    //   dy of K-tile t+1 (its stage was last read in slot -1): first group from its M0 (slot 0), second from its previous C1 (slot 0);
+    //     waited for before the end of slot 3 (first group's C1, second group's M1), read from slot 4 on
+    //   codes of K-tile t+1: converted and written in C0 (slots 1 and 2), waited for in M1; the codes of K-tile t+2 are loaded then
+    // (K-tiles past the end are written into a stage that nothing reads any more).
+    // A wave's vector-memory instructions retire in order and every C0 issues four loads behind the dy of its K-tile, so vmcnt(4)
+    // waits for dy and leaves the codes in flight.
+    auto half = [&](auto second_tag) {
+      constexpr bool SECOND = decltype(second_tag)::value;
+      constexpr int NB = SECOND ? NF - NFW : NFW;
+      G2Frags<1, 4> fa;
+      G2Frags<1, NB> fb;
+      fa.init(wm * 4, 0, lane);
+      fb.init(SECOND ? NFW : 0, BOFF, lane);
+      bf16x8 af[4], bf[NB];
+      auto dma = [&](__amdgpu_buffer_rsrc_t rs, int t, int i) { la.issue(rs, true, i, smem + (t & 1) * STAGE, wave); };      // piece i
+#define W8_SLOT_END() do { __builtin_amdgcn_sched_barrier(0); __builtin_amdgcn_s_barrier(); __builtin_amdgcn_sched_barrier(0); } while (0)
+#define W8_READ(KS)                                              \
+  fa.template read_range<KS, true, 0, 4, 4>(smem, af);           \
+  fb.template read_range<KS, true, 0, NB, NB>(smem, bf);
+      if (SECOND) {
+        const __amdgpu_buffer_rsrc_t rs = a_rsrc(1);
 #pragma unroll
-      for (int j = 0; j < NFW; ++j) {
-        W8_MFMA_GROUP(j, a1, b1);
-        __builtin_amdgcn_sched_barrier(0);
-        // under the matrix instructions just issued: K-tile t+2's codes and dy, the fragments of K-tile t+1's first half
-        if (j < 2) { b_write(t & 1, j, qv[j], sv[j]); b_load(t + 3, j, qv[j], sv[j]); }
-        if (j < 2) { la.issue(ra, true, 2 * j, st, wave); la.issue(ra, true, 2 * j + 1, st, wave); }
-        if (j == 1) { W8_READ_A(0, a0); }
-        if (j == 2) { W8_READ_B(0, b0, 0, 4); }
-        if (j == 3) { W8_READ_B(0, b0, 4, NFW); }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < PA; ++i) dma(rs, 1, i);
+        W8_SLOT_END();
       }
-    }
-    W8_PHASE1();
-    W8_WAIT_FRAGS();
+      for (int t = 0; t < nkt; ++t) {
+        // M0
+        W8_READ(0);
+        if (!SECOND) {
+          const __amdgpu_buffer_rsrc_t ra = a_rsrc(t + 1);
 #pragma unroll
-    for (int j = 0; j < NFW; ++j) { W8_MFMA_GROUP(j, a1, b1); }
-#undef W8_PHASE1
-#undef W8_WAIT_FRAGS
-#undef W8_MFMA_GROUP
-#undef W8_READ_A
-#undef W8_READ_B
+          for (int i = 0; i < PA; ++i) dma(ra, t + 1, i);
+        }
+        __builtin_amdgcn_s_waitcnt(0xc07f);    // lgkmcnt(0): the fragments (the compiler cannot see those reads)
+        W8_SLOT_END();
+        // C0; operands swapped: a lane ends up with 4 neighbouring columns of one row
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int x = 0; x < 4 * NB; ++x) {
+          acc[x & 3][x >> 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[x >> 2], af[x & 3], acc[x & 3][x >> 2], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          if (x < 6) b_step((t + 1) & 1, 0, x);
+          if (x == 6) b_load(q_rsrc(t + 2), s_rsrc(t + 2), 0);
+          if (x >= 7 && x < 13) b_step((t + 1) & 1, 1, x - 7);
+          if (x == 13) b_load(q_rsrc(t + 2), s_rsrc(t + 2), 1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        W8_SLOT_END();
+        // M1
+        W8_READ(1);
+        __builtin_amdgcn_s_waitcnt(SECOND ? 0x0074 : 0xc07f);      // lgkmcnt(0); second group: and dy of K-tile t+1, vmcnt(4)
+        W8_SLOT_END();
+        // C1
+        const __amdgpu_buffer_rsrc_t ra = a_rsrc(t + 2);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int x = 0; x < 4 * NB; ++x) {
+          acc[x & 3][x >> 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[x >> 2], af[x & 3], acc[x & 3][x >> 2], 0, 0, 0);
+          if (SECOND && (x & 3) == 1 && (x >> 2) < PA) { __builtin_amdgcn_sched_barrier(0); dma(ra, t + 2, x >> 2); __builtin_amdgcn_sched_barrier(0); }
+        }
+        __builtin_amdgcn_s_setprio(0);
+        if (!SECOND) __builtin_amdgcn_s_waitcnt(0x0f74);           // dy of K-tile t+1
+        W8_SLOT_END();
+        fa.toggle((t & 1) ? -STAGE : STAGE); fb.toggle((t & 1) ? -STAGE : STAGE);
+      }
+      if (!SECOND) W8_SLOT_END();
+#undef W8_SLOT_END
+#undef W8_READ
+    };
+    if (wn == 0) half(std::false_type{}); else half(std::true_type{});
     __builtin_amdgcn_s_waitcnt(0x0070);      // no LDS-DMA (of the K-tile past the end) outlives its part, or the workgroup
 
     // lane: row lane & 15, columns 4 (lane >> 4) .. + 3 of each 16 x 16 fragment
@@ -301,8 +333,8 @@ __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const Wgrad8Params
 
 // ---- host
 struct Wgrad8Plan { int nf, grid, whole, cut, cut_tiles, piece, pieces; int64_t slots; };
-// The cheapest of the tile widths and cuts, in microseconds of the longest workgroup: K-tiles (measured 1.36 us at 128 columns, 1.48
-// at 208, 1.6 at 256), start and end of each part, and the parts' way to the workspace and back over the whole chip
+// The cheapest of the tile widths and cuts, in microseconds of the longest workgroup: K-tiles (measured 1.30 us at 128 columns, 1.38
+// at 208, 1.53 at 256), start and end of each part, and the parts' way to the workspace and back over the whole chip
 // (256 x 16 nf floats written and read at 5 TB/s) with the join's launch and the depth of its sums.
 static Wgrad8Plan w8_plan(int64_t m, int64_t n, int64_t k) {
   const int64_t tm = (m + 255) / 256, kt = (k + G2_BK - 1) / G2_BK;
@@ -321,7 +353,7 @@ static Wgrad8Plan w8_plan(int64_t m, int64_t n, int64_t k) {
       if (piece < 4) piece = kt < 4 ? kt : 4;            // <= kt always: a piece lies in two tiles at most
       const int64_t pieces = (line + piece - 1) / piece;
       const int64_t slots = (cut > 1 ? ct * cut : 0) + (line ? pieces + (left - ct) : 0);
-      const double kt_us = nf == 8 ? 1.36 : nf == 13 ? 1.48 : 1.6;
+      const double kt_us = nf == 8 ? 1.30 : nf == 13 ? 1.38 : 1.53;
       const double longest = (double)(whole / W8_WGS) * (kt * kt_us + 4) + (left ? (kt + cut - 1) / cut * kt_us + 4 : 0) +
                              (line ? piece * kt_us + 4 : 0);
       const double depth = line ? (double)kt / piece : (double)cut;
