@@ -434,6 +434,30 @@ def test_offsets_beyond_32_bits(ops):
     assert torch.equal(dx[-5:], ops.addnorm_bwd(tail, few.act, few.rstd, dx_dtype=BF16, want_dgamma=False)[0])
 
 
+@pytest.mark.parametrize("which", ["dy", "codes"])
+def test_wgrad_over_more_than_2_gib(ops, which):
+    """Rows 2 MiB (dy) or 1 MiB (codes) apart: the sum needs more than one call of the kernel; pads of dy hold NaN."""
+    k, m, n, pitch = 2600, 40, 100, 1 << 20
+    x, dy = rows_of(k, n, F32, 1.0, 3), rows_of(k, m, BF16, 1.0, 5)
+    a = ops.act8_pack(x)
+    want, start = ops.act8_wgrad(dy, a), torch.randn(m, n, generator=torch.Generator().manual_seed(6)).cuda()
+    if which == "dy":
+        far = torch.empty(k, pitch, dtype=BF16, device="cuda")
+        far[:, m:m + 8] = float("nan")
+        far[:, :m] = dy
+        got, acc = ops.act8_wgrad(far[:, :m], a), ops.act8_wgrad(far[:, :m], a, out=start.clone())
+    else:
+        q = torch.empty(k, pitch, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+        q.view(torch.uint8)[:, :128] = a.q.view(torch.uint8)
+        far = ops.Act8(q[:, :128], a.scale, n)
+        got, acc = ops.act8_wgrad(dy, far), ops.act8_wgrad(dy, far, out=start.clone())
+    v, d = R.values(a), dy.cpu().double()
+    tol = (8 * k ** 0.5 + 8) * U * (d.abs().t() @ v.abs()) + 1e-30
+    close(got, d.t() @ v, tol)
+    close(want, d.t() @ v, tol)
+    close(acc, start.cpu().double() + d.t() @ v, tol + 8 * U * start.cpu().double().abs())
+
+
 def test_refusals_on_the_device(ops):
     x = torch.zeros(4, 64, device="cuda")
     with pytest.raises(ValueError, match="16-byte"):

@@ -540,11 +540,16 @@ def act8_wgrad(dy, act: Act8, out=None):
         raise ValueError(f"vita_amd: out has shape {tuple(out.shape)}, expected {(m, n)}")
     _vec(out, "out", m * n)
     dw = torch.empty(m, n, dtype=torch.float32, device=dy.device) if out is None else out
-    ws_bytes = _lib.lib().vita_act8_wgrad_ws_bytes(m, n, k)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device) if ws_bytes else None
+    qp, ldq, sp, lds = q
+    # the kernel's offsets inside a call are 32 bits: longer sums go in several calls (whole K-tiles, five of them to spare)
+    most = max(0x7ffffe00 // max(2 * ld, ldq, lds) // 64 * 64 - 320, 64)
     with _Timed("act8_wgrad", 2.0 * m * n * k):
-        check(_lib.lib().vita_act8_wgrad(dy.data_ptr(), ld, *q, dw.data_ptr(), n, m, n, k, int(out is not None), _p(ws),
-                                           ws_bytes, _s()), "act8_wgrad")
+        for r in range(0, k, most):
+            rows = min(most, k - r)
+            ws_bytes = _lib.lib().vita_act8_wgrad_ws_bytes(m, n, rows)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device) if ws_bytes else None
+            check(_lib.lib().vita_act8_wgrad(dy.data_ptr() + 2 * r * ld, ld, qp + r * ldq, ldq, sp + r * lds, lds, dw.data_ptr(), n, m, n,
+                                             rows, int(out is not None or r > 0), _p(ws), ws_bytes, _s()), "act8_wgrad")
     return dw
 
 
