@@ -298,6 +298,17 @@ def test_add_rms_norm_layouts_and_refusals(V):
     assert torch.equal(torch.autograd.grad(y.square().sum(), x8)[0], want)
 
 
+def test_second_derivatives_are_refused(V):
+    """The backward passes are kernels too and have no gradient of their own: an error, not a sum with that part missing."""
+    x = torch.randn(2, 5, 64, device="cuda", requires_grad=True)
+    norm = nn.RMSNorm(64).cuda()
+    blk = make_block(V, 64, 2, "layer", 8)
+    for f in (lambda: V.add_rms_norm(x, x, norm.weight)[0], lambda: V.layer_norm_padded(x, norm), lambda: blk.forward_padded(x)):
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            torch.autograd.grad(f().square().sum(), x, create_graph=True)
+        torch.autograd.grad(f().square().sum(), x)
+
+
 def test_training_pass_in_a_graph(V):
     """Forward and backward of a chain of norms captured once, replayed on new inputs: each replay equals eager."""
     x = torch.randn(40, 205, device="cuda").to(BF16).requires_grad_()

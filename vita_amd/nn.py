@@ -11,6 +11,7 @@ Data layout in HBM:
 """
 from __future__ import annotations
 
+import functools
 import math
 import os
 import weakref
@@ -547,6 +548,16 @@ def norm_bwd_padded(dy, src, rstd, ln, D, Dp, need_w, need_b, dx_in=None):
     return dx, dxb, dw, db
 
 
+def _first_order(backward):
+    """For backward passes that are kernels: refuses create_graph=True, where their part would be missing from the second derivative."""
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        if torch.is_grad_enabled():
+            raise RuntimeError("vita_amd: these kernels have no second derivatives (create_graph=True)")
+        return backward(ctx, *grads)
+    return run
+
+
 class _BlockActFn(torch.autograd.Function):
     """The Block with RMS norms and / or with its activations kept in 8 bits (saved_bits=8).  What the backward pass keeps of a
     token then: the two norms' normalised rows (from which their own gradients AND the weight gradients of the products behind
@@ -596,6 +607,7 @@ class _BlockActFn(torch.autograd.Function):
         return x2.view(B, N, Dp)
 
     @staticmethod
+    @_first_order
     def backward(ctx, dx2):
         blk = ctx.blk
         dm: Dims = blk.dims
@@ -767,6 +779,7 @@ class _NormActFn(torch.autograd.Function):
         return a.y.view(B, N, Dp)
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy):
         ln = ctx.ln
         B, N, Dp = dy.shape
@@ -802,6 +815,7 @@ class _AddRmsNormFn(torch.autograd.Function):
         return y, s
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy, ds):
         shape, xt, rt, bits = ctx.meta
         D = shape[-1]
