@@ -16,11 +16,13 @@
 //   * a part of a tile goes to the workspace as fp32; a second kernel adds a tile's parts in their order.  One writer per
 //     element, no atomics: the same bits on every call.
 //
-// Measured (MI355X): 3776 tokens, 1025 x 4100: 42 + 15 us (join), 750 TFLOP/s without the join; 13826 tokens, 1025 x 3075: 109 + 15 us,
+// Measured (MI355X): 3776 tokens, 1025 x 4100: 42 + 13 us (join), 750 TFLOP/s without the join; 13826 tokens, 1025 x 3075: 109 + 13 us,
 // 800 TFLOP/s; the bf16 kernel of gemm256.hip with atomics takes 85 and 131 us for the same shapes, without the pass that restores its
 // operand.  Bound by what one wave after another can issue: without the conversions 98 us of the 109 are left, without the DMA of dy
 // 96, without either 85 (matrix instructions, fragment reads, barriers); without the loads of the codes 109.  With all waves in step and
-// the conversions in one piece behind the barrier the two shapes take 43 and 114 to 122 us; with four waves of twice the rows 124.
+// the conversions in one piece behind the barrier the two shapes take 43 and 114 to 122 us; with four waves of twice the rows 124; when
+// in the K-tile the DMA is issued makes no difference.  8 of the 42 us are the writing of the parts (in fragment order or not alike,
+// non-temporal 12); 15 us the join with single floats stored.
 #include "act8.h"
 #include "gemm256.h"
 #include <type_traits>
@@ -53,6 +55,19 @@ __device__ __forceinline__ int64_t w8_piece_slot(const Wgrad8Params& P, int piec
   return (int64_t)P.cut_tiles * P.cut + 2 * piece + second;
 }
 __device__ __forceinline__ int w8_cut_begin(const Wgrad8Params& P, int part) { return (int)((int64_t)P.kt * part / P.cut); }
+
+// 4 neighbouring columns of a row of dw, `left` of them inside; rows start on any 4-byte boundary, which 16-byte stores take too
+__device__ __forceinline__ void w8_put(const Wgrad8Params& P, float* o, f32x4 v, int64_t left) {
+  typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+  if (left >= 4) {
+    if (P.accumulate) v += *reinterpret_cast<const f32x4_any*>(o);
+    *reinterpret_cast<f32x4_any*>(o) = v;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 3; ++r)
+      if (r < left) o[r] = P.accumulate ? o[r] + v[r] : v[r];
+  }
+}
 
 __device__ __forceinline__ uint64_t w8_uniform(uint64_t v) { return ((uint64_t)g2_sgpr((uint32_t)(v >> 32)) << 32) | g2_sgpr((uint32_t)v); }
 // descriptor of the bytes [adv, bytes) behind base; operands uniform and below 2^31 (the host checks them).  The maximum is a signed one
@@ -279,11 +294,8 @@ __global__ __launch_bounds__(G2_THREADS, 2) void act8_wgrad_kernel(const Wgrad8P
 #pragma unroll
         for (int j = 0; j < NFW; ++j) {
           if (j >= nfw) continue;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int64_t col = n0 + cl + 16 * j + r;
-            if (col < P.n) o[col] = P.accumulate ? o[col] + acc[i][j][r] : acc[i][j][r];
-          }
+          const int64_t col = n0 + cl + 16 * j;
+          w8_put(P, o + col, acc[i][j], P.n - col);
         }
       }
     } else {
@@ -297,6 +309,19 @@ __global__ __launch_bounds__(G2_THREADS, 2) void act8_wgrad_kernel(const Wgrad8P
   }
 }
 
+// s + p[0] + p[step] + ... + p[(n - 1) step], eight loads in flight
+__device__ __forceinline__ f32x4 w8_sum_parts(const float* p, int n, int64_t step, f32x4 s) {
+  for (int i = 0; i < n; i += 8) {
+    f32x4 t[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i + u < n) t[u] = *reinterpret_cast<const f32x4*>(p + (i + u) * step);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i + u < n) s += t[u];
+  }
+  return s;
+}
 // adds the parts of each tile that was cut, in their order: grid (tiles behind the whole ones, quads of a tile / 256); a thread owns
 // 4 neighbouring columns of a row
 __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const Wgrad8Params P, const int width) {
@@ -313,22 +338,15 @@ __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const Wgrad8Params
   f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
   if (blockIdx.x < (unsigned)P.cut_tiles) {
     if (P.cut == 1) return;                              // written already
-    p += w8_cut_slot(P, tile, 0) * slot_floats;
-#pragma unroll 8
-    for (int i = 0; i < P.cut; ++i) s += *reinterpret_cast<const f32x4*>(p + i * slot_floats);
+    s = w8_sum_parts(p + w8_cut_slot(P, tile, 0) * slot_floats, P.cut, slot_floats, s);
   } else {
     const int64_t t0 = (int64_t)(blockIdx.x - P.cut_tiles) * P.kt, t1 = t0 + P.kt;
     const int w0 = (int)(t0 / P.piece), w1 = (int)((t1 + P.piece - 1) / P.piece);
     if ((int64_t)w0 * P.piece < t0) s = *reinterpret_cast<const f32x4*>(p + w8_piece_slot(P, w0, 1) * slot_floats);
     else s = *reinterpret_cast<const f32x4*>(p + w8_piece_slot(P, w0, 0) * slot_floats);
-    p += w8_piece_slot(P, w0 + 1, 0) * slot_floats;
-#pragma unroll 8
-    for (int i = 0; i < w1 - w0 - 1; ++i) s += *reinterpret_cast<const f32x4*>(p + 2 * i * slot_floats);
+    s = w8_sum_parts(p + w8_piece_slot(P, w0 + 1, 0) * slot_floats, w1 - w0 - 1, 2 * slot_floats, s);
   }
-  float* o = P.dw + row * P.lddw + col;
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (col + r < P.n) o[r] = P.accumulate ? o[r] + s[r] : s[r];
+  w8_put(P, P.dw + row * P.lddw + col, s, P.n - col);
 }
 
 // ---- host
