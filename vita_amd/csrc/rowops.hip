@@ -669,6 +669,11 @@ __global__ __launch_bounds__(256) void colsum_kernel(const void* __restrict__ x,
     }
   }
 }
+// a kernel, not hipMemsetAsync: replays of a captured graph ran that out of its place
+__global__ __launch_bounds__(256) void fill_zero_kernel(float* __restrict__ p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = 0.f;
+}
 static int colsum_impl(const void* x, int32_t dtype, int64_t ld, int64_t rows, int64_t cols, float* out, bool zero, void* stream);
 extern "C" int vita_colsum(const void* x, int32_t dtype, int64_t ld, int64_t rows, int64_t cols, float* out, void* stream) {
   return colsum_impl(x, dtype, ld, rows, cols, out, true, stream);
@@ -681,7 +686,10 @@ static int colsum_impl(const void* x, int32_t dtype, int64_t ld, int64_t rows, i
   const int cpt = f32 ? 4 : 8;
   VITA_REQUIRE(x && out && rows > 0 && cols > 0 && ld % cpt == 0 && ld >= ((cols + cpt - 1) / cpt) * cpt);
   VITA_REQUIRE(((uintptr_t)x & 15) == 0);
-  if (zero && hipMemsetAsync(out, 0, cols * sizeof(float), (hipStream_t)stream) != hipSuccess) return VITA_ERR_LAUNCH;
+  if (zero) {
+    hipLaunchKernelGGL(fill_zero_kernel, dim3((unsigned)((cols + 255) / 256)), dim3(256), 0, (hipStream_t)stream, out, cols);
+    VITA_CHECK_LAUNCH("vita_colsum_zero");
+  }
   const int64_t colblk = (cols + 16 * cpt - 1) / (16 * cpt);
   // about 2048 blocks in all (8 per CU), at least 128 rows per block (one batch of 8 loads per thread), at most 256 row
   // chunks: every chunk ends in one fp32 atomic per column
