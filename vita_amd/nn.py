@@ -329,7 +329,9 @@ class _SideStream:
     to a main-stream allocation while the side stream still uses it."""
 
     def __init__(self, device, enabled=True):
-        self.on = bool(enabled and WGRAD_SIDE_STREAM)
+        # under capture everything stays on the capturing stream: a captured graph of two streams with several forks from one node has
+        # been replayed with kernels before the ones they wait for (seen with plain element-wise kernels too)
+        self.on = bool(enabled and WGRAD_SIDE_STREAM and not torch.cuda.is_current_stream_capturing())
         if not self.on:
             return
         global _DEFERRED_DONE
