@@ -203,9 +203,12 @@ extern "C" int vita_addnorm_fwd(const vita_addnorm_fwd_desc* dp, void* stream) {
       if (rt == 0) AN_LAUNCH(W, NV, T, false, 0); else if (rt == 1) AN_LAUNCH(W, NV, T, false, 1); else AN_LAUNCH(W, NV, T, false, 2);      \
     }                                                                                                                                        \
   } while (0)
-  // few rows: four waves to a row shorten the way through one row
+  // Few rows: four waves to a row shorten the way through one row, many rows: a wave to each saves the barriers.  One wave / four, us,
+  // bf16 + fp32 residual, 600 columns: 1 row 3.7 / 3.0, 512 rows 5.3 / 4.8, 1024 5.8 / 6.0, 2048 7.0 / 8.7; 1025 columns: 3.8 / 3.2,
+  // 5.6 / 5.2, 6.2 / 6.3, 8.3 / 9.7.  Above 1536 columns a wave would hold 4 chunks and more (64 registers of values): four waves, with
+  // one chunk a lane as far as that goes (2000 columns, 8192 rows: 34.0 us, with two chunks, half of them empty, 36.6).
   if (width <= 512) AN_TYPES(1, 1, false);
-  else if (width <= 2048 && D.rows <= AN_FEW_ROWS) AN_TYPES(4, 1, false);
+  else if (width <= 2048 && (D.rows <= AN_FEW_ROWS || width > 1536)) AN_TYPES(4, 1, false);
   else if (width <= 1024) AN_TYPES(1, 2, false);
   else if (width <= 1088) AN_TYPES(1, 2, true);
   else if (width <= 1536) AN_TYPES(1, 3, false);
@@ -450,10 +453,13 @@ extern "C" int vita_addnorm_bwd(const vita_addnorm_bwd_desc* dp, void* stream) {
       if (src == 0) AN_LAUNCH(W, NV, T, 0, false); else if (src == 1) AN_LAUNCH(W, NV, T, 1, false); else AN_LAUNCH(W, NV, T, 2, false);    \
     }                                                                                                                                        \
   } while (0)
+  // One wave a row up to 1536 columns, four beyond, us from 8 bits, fp32 dx_in and dx: 1025 columns, 30000 rows: 70 with one, 121 with
+  // four; 2000 columns: 140 with four of one chunk, 158 of two (half of them empty).
   if (width <= 512) AN_TYPES(1, 1, false);
   else if (width <= 1024) AN_TYPES(1, 2, false);
   else if (width <= 1088) AN_TYPES(1, 2, true);
   else if (width <= 1536) AN_TYPES(1, 3, false);
+  else if (width <= 2048) AN_TYPES(4, 1, false);
   else if (width <= 4096) AN_TYPES(4, 2, false);
   else AN_TYPES(4, 4, false);
 #undef AN_TYPES
