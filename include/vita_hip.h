@@ -229,7 +229,8 @@ int vita_attn_bwd(const void* qkv, const void* o, const void* dout, const float*
  * scale: uint8 [rows][lds], ceil(d / 32) bytes of a row are written.  Readers take bytes 10..246, which is what the writers
  * below produce; other bytes are read without harm, their values are not specified.
  * d <= 2^20; empty matrices are refused.  Matrices of dtype VITA_DT_BF16 need ld % 8 == 0, fp32 ld % 4 == 0, both 16-byte
- * alignment; columns [d, ld) of an output are written as zero, columns >= d of an input are never read. */
+ * alignment; columns [d, ld) of an output are written as zero, what stands in columns >= d of an input does not matter (nothing
+ * outside the memory from a matrix' first to its last element is read). */
 int vita_act8_pack(const void* x, int32_t dtype, int64_t ldx, int64_t rows, int64_t d, void* q, int64_t ldq, void* scale,
                    int64_t lds, void* stream);
 /* y = value, or value * gamma (+ beta) per column (gamma, beta fp32 [d] or NULL): a norm's output from its normalised rows */

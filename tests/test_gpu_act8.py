@@ -331,6 +331,31 @@ def test_addnorm_bwd_types(ops, kind, src, dyt, dxt, with_in):
     _check_bwd(ops, 23, 205, kind, src, dyt, dxt, with_in, 5, gamma=with_in)
 
 
+@pytest.mark.parametrize("rows,d", [(1, 5), (2, 5), (3, 5), (40, 5), (41, 69), (33, 130), (33, 250), (70, 300), (40, 777), (40, 1601), (40, 2636),
+                                    (40, 3500), (40, 5001), (40, 7003)])
+def test_rows_that_end_inside_a_chunk(ops, rows, d):
+    """Every way a row is held, with a last chunk of 8 columns that is not whole: against the formulas, and the same bits on rows
+    without room between them (fp32 rows 4 columns apart reach into the next row) as on rows far apart."""
+    _check_bwd(ops, rows, d, "layer", "act8", F32, BF16, True, rows + d)
+    _check_bwd(ops, rows, d, "rms", "f32", BF16, F32, True, rows + d)
+    x, res, gamma, beta = _norm_case(rows, d, F32, BF16, "layer", rows + d)
+    a, _ = _check_norm(ops, x, res, gamma, beta, "layer", 1e-5, F32, BF16, "output")
+    tight = lambda t, step: rows_of(rows, d, t.dtype, 1.0, 0, step=step).copy_(t)
+    same = lambda u, v: all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(u, v))
+    b = ops.addnorm_fwd(tight(x, 4), gamma, beta, residual=tight(res, 64), kind="layer", eps=1e-5, y_dtype=F32, sum_dtype=BF16, pack="output")
+    assert same((a.y, a.sum, a.act.q, a.act.scale, a.rstd, a.mean), (b.y, b.sum, b.act.q, b.act.scale, b.rstd, b.mean))
+    dy = rows_of(rows, d, F32, 1.0, d)
+    f = lambda k: ops.addnorm_bwd(tight(dy, k), tight(x, k), a.rstd, gamma, kind="layer", mean=a.mean, dx_in=tight(dy, k))
+    assert same(f(4), f(64))
+    z = rows_of(rows, d, BF16, 1.0, d + 1)
+    for u, v in ((x, 4), (z, 8)):
+        p, q = ops.act8_pack(tight(u, v)), ops.act8_pack(tight(u, 64))
+        assert same(p[:2], q[:2])
+        (g, p), (h, q) = ops.gelu_act8_fwd(tight(u, v)), ops.gelu_act8_fwd(tight(u, 64))
+        assert same((g,) + p[:2], (h,) + q[:2])
+    assert same(ops.gelu_act8_bwd(tight(z, 8), p), ops.gelu_act8_bwd(tight(z, 64), p))
+
+
 @pytest.mark.parametrize("kind", ["rms", "layer"])
 def test_addnorm_gradient_against_differences(ops, kind):
     """dx and dgamma from the kept sum against central differences of the 64-bit forward formula."""

@@ -83,13 +83,14 @@ __device__ __forceinline__ void act8_decode(u32x2 q, uint32_t byte, float (&v)[8
   }
 }
 
-// ---- 8 neighbouring columns [c, c + 8) of a row with d real columns; columns >= d read as 0 and are never touched
+// ---- 8 neighbouring columns [c, c + 8) of a row with d real columns; columns >= d read as 0 and are never touched.  whole: the row has
+// two more behind it, so that all 8 are inside the matrix' memory wherever c < d; what stands behind d comes back as it is then.
 struct Raw8 { u32x4 a, b; };      // bf16 rows use a only
 template <bool F32>
-__device__ __forceinline__ Raw8 raw_load8(const void* row, int c, int d) {
+__device__ __forceinline__ Raw8 raw_load8(const void* row, int c, int d, bool whole = false) {
   Raw8 w;
   w.a = w.b = u32x4{0, 0, 0, 0};
-  if (c + 8 <= d) {
+  if (c + 8 <= d || (whole && c < d)) {
     if (F32) {
       w.a = *reinterpret_cast<const u32x4*>((const float*)row + c);
       w.b = *reinterpret_cast<const u32x4*>((const float*)row + c + 4);

@@ -4,7 +4,7 @@
 // threads in order, so that narrow, wide and odd rows fill the chip alike.  One chunk to a thread: two or four with their loads
 // together are no faster (GELU backward 46082 x 4100: 250, 264, 284 us).  Measured (MI355X, kernels alone; a copy reaches 5 TB/s):
 //   pack 13826 x 1025 fp32 13 us (5.4 TB/s); restore it with gamma and beta 12 us (one load for each element of gamma: 55 us)
-//   GELU forward 13826 x 4100 60 us (4.8 TB/s), 3776 x 4100 18 us; backward 46082 x 4100 250 us (5.3 TB/s), 3776 x 4100 22 us (about 36
+//   GELU forward 13826 x 4100 55 us (5.2 TB/s), 3776 x 4100 17 us; backward 46082 x 4100 246 us (5.4 TB/s), 3776 x 4100 21 us (about 36
 //   issue slots an element, 8 of them exp and rcp: two thirds of the time at this size)
 #include "act8.h"
 
@@ -14,6 +14,16 @@ __device__ __forceinline__ void codes_load8(const uint8_t* q, const uint8_t* sca
   uint32_t byte = 127;
   if (c < d) { w = *reinterpret_cast<const u32x2*>(q + c); byte = scale[c >> 5]; }
   act8_decode(w, byte, v);
+}
+
+// 8 neighbouring columns of a row as floats, zeros behind the row's end (whole: see raw_load8)
+template <bool F32>
+__device__ __forceinline__ void row_load8(const void* row, int c, int d, bool whole, float (&v)[8]) {
+  raw_values8<F32>(raw_load8<F32>(row, c, d, whole), v);
+  if (c + 8 > d) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) if (c + r >= d) v[r] = 0.f;
+  }
 }
 
 struct ChunkMap {      // chunk number -> (row, column) for rows of nc chunks
@@ -48,7 +58,7 @@ __global__ __launch_bounds__(A8_THREADS) void act8_pack_kernel(const void* __res
                                                                int64_t lds) {
   for_chunk(M, [&](int64_t row, int c) {
     float v[8];
-    raw_values8<F32>(raw_load8<F32>((const char*)x + row * ldx * (F32 ? 4 : 2), c, d), v);
+    row_load8<F32>((const char*)x + row * ldx * (F32 ? 4 : 2), c, d, row + 2 < M.rows, v);
     uint32_t byte;
     const u32x2 w = act8_encode(v, byte);
     *reinterpret_cast<u32x2*>(q + row * ldq + c) = w;
@@ -119,7 +129,7 @@ __global__ __launch_bounds__(A8_THREADS) void gelu_act8_fwd_kernel(const void* _
                                                                    int64_t ldq, uint8_t* __restrict__ scale, int64_t lds) {
   for_chunk(M, [&](int64_t row, int c) {
     float v[8];
-    raw_values8<F32>(raw_load8<F32>((const char*)z + row * ldz * (F32 ? 4 : 2), c, d), v);
+    row_load8<F32>((const char*)z + row * ldz * (F32 ? 4 : 2), c, d, row + 2 < M.rows, v);
     uint32_t byte;
     const u32x2 w = act8_encode(v, byte);
     if (c < d + 31 - (d + 31) % 32) {      // d rounded up to whole groups
@@ -157,7 +167,7 @@ __global__ __launch_bounds__(A8_THREADS) void gelu_act8_bwd_kernel(const uint16_
                                                                    uint16_t* __restrict__ g, int64_t ldg) {
   for_chunk(M, [&](int64_t row, int c) {
     float v[8], t[8], p[8];
-    raw_values8<false>(raw_load8<false>(dg + row * lddg, c, d), t);
+    raw_values8<false>(raw_load8<false>(dg + row * lddg, c, d, row + 2 < M.rows), t);
     codes_load8(q + row * ldq, scale + row * lds, c, d, v);
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
@@ -165,7 +175,7 @@ __global__ __launch_bounds__(A8_THREADS) void gelu_act8_bwd_kernel(const uint16_
       gelu_erf_both(v[r], p[r], der);
       t[r] *= der;
     }
-    if (c + 8 > d) {                        // codes behind d are whatever the caller's buffer holds
+    if (c + 8 > d) {                        // codes and dg behind d are whatever the caller's buffers hold
 #pragma unroll
       for (int r = 0; r < 8; ++r) if (c + r >= d) t[r] = p[r] = 0.f;
     }

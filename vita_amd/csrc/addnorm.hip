@@ -9,13 +9,16 @@
 // n comes from the 8-bit rows (1.03 bytes a value and rstd) or from s and (mu, rstd).
 //
 // Both move bytes.  Measured (MI355X, kernels alone; a copy of that size reaches 5 TB/s):
-//   forward, 46082 x 1025, bf16 + fp32 -> fp32 sum, bf16 y, 8-bit n: 134 us, 4.6 TB/s (one wave per row and a row per block of gamma
+//   forward, 46082 x 1025, bf16 + fp32 -> fp32 sum, bf16 y, 8-bit n: 133 us, 4.8 TB/s (one wave per row and a row per block of gamma
 //     and beta loads: 186 us; rows dealt to resident waves with gamma in registers: 141 us; 64 columns behind the chunks one to a
 //     lane: 134 us)
-//   backward, 13826 x 1025, from 8 bits, bf16 dy, fp32 dx_in and dx: 38 + 4 us (sums of the partial rows), 4.1 TB/s (gamma read
+//   backward, 13826 x 1025, from 8 bits, bf16 dy, fp32 dx_in and dx: 37 + 4 us (sums of the partial rows), 4.5 TB/s (gamma read
 //     anew for each row and dx_in after the sums: 89 + 16 us; loads together, gamma in registers: 61; 768 partial rows of 1025
-//     columns added with all loads in flight: 4 instead of 16 us; last columns one to a lane, 3 blocks a CU instead of 2: 38)
-//   backward, 4096 x 4096, from a bf16 sum: 33 + 4 us, 4.1 TB/s (62 + 13 us before)
+//     columns added with all loads in flight: 4 instead of 16 us; last columns one to a lane, 3 blocks a CU instead of 2: 37; with
+//     fp32 dy the compiler has to be held to the registers of 3 blocks: 46082 rows 118 -> 88 us)
+//   backward, 4096 x 4096, from a bf16 sum: 30 + 4 us (four waves with two chunks a lane instead of eight with one: 33)
+//   rows whose last chunk is not whole, loaded in one piece instead of by columns: 46082 x 777 backward 80 -> 63 us, 29000 x 1601
+//     forward 162 -> 133, backward 132 -> 93
 #include "act8.h"
 
 #define AN_RMS 0
@@ -23,12 +26,15 @@
 #define AN_MAX_D 8192
 #define AN_FWD_MAXBLK 2048
 #define AN_FEW_ROWS 1024
+// how a wave holds a row: its 64 lanes; those and one column a lane more; or (16, 32) that many lanes of it
+#define AN_FULL 0
+#define AN_TAIL 1
 
-// sums over the W waves that share a row (W = 1: the wave itself, no barrier), two at a time
-template <int W>
+// sums over the W waves that share a row (W = 1: the wave itself, or its L neighbouring lanes, no barrier), two at a time
+template <int W, int L>
 __device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2][W], int& turn, int wave, int lane) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
+  for (int o = L / 2; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
   if (W == 1) return;
   turn ^= 1;                          // two slots in turn: the barrier of the next sum lies between a slot's reads and its next writes
   if (lane == 0) { red[turn][0][wave] = a; red[turn][1][wave] = b; }
@@ -37,9 +43,10 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2][W],
 #pragma unroll
   for (int w = 1; w < W; ++w) { a += red[turn][0][w]; b += red[turn][1][w]; }
 }
-template <int W>
+template <int W, int L>
 __device__ __forceinline__ float row_sum(float a, float (*red)[2][W], int& turn, int wave, int lane) {
-  a = wave_sum(a);
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) a += __shfl_xor(a, o, 64);
   if (W == 1) return a;
   turn ^= 1;
   if (lane == 0) red[turn][0][wave] = a;
@@ -53,12 +60,14 @@ __device__ __forceinline__ float row_sum(float a, float (*red)[2][W], int& turn,
 // A wave (W = 1) or the four waves of a block (W = 4) walk over rows, 8 neighbouring columns to a lane and chunk, the row in
 // registers from its loads to its stores; gamma and beta stay in registers.  T: up to 64 columns behind the last whole chunk go one to
 // a lane instead of opening another chunk (1025 columns would fill 1 of its 64 lanes and cost every lane 8 columns of registers and
-// arithmetic; measured below).
-template <int W, int NV, bool T, bool XF, int RT>      // RT: 0 no residual, 1 bf16, 2 fp32
-__global__ __launch_bounds__(256) void addnorm_fwd_kernel(const vita_addnorm_fwd_desc D, const int al) {
+// arithmetic).  M = 16, 32: narrow rows, 4 or 2 of them to a wave.
+template <int W, int NV, int M, bool XF, int RT>      // RT: 0 no residual, 1 bf16, 2 fp32
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void addnorm_fwd_kernel(const vita_addnorm_fwd_desc D, const int al) {
+  constexpr bool T = M == AN_TAIL;
+  constexpr int L = M > AN_TAIL ? M : 64, R = W == 1 ? 256 / L : 1;      // lanes of a wave to a row; rows of a block at a time
   __shared__ float red[2][2][W];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int d = (int)D.d, t0 = (W == 1 ? lane : (int)threadIdx.x) * 8;
+  const int d = (int)D.d, t0 = (W == 1 ? lane % L : (int)threadIdx.x) * 8;
   const double inv_d = 1.0 / (double)d;
   int turn = 0;
   float gm[NV][8], bt[NV][8];
@@ -69,14 +78,15 @@ __global__ __launch_bounds__(256) void addnorm_fwd_kernel(const vita_addnorm_fwd
   }
   const int ct = NV * 512 + lane;                // the lane's column behind the chunks
   const float gt = T && ct < d && D.gamma ? D.gamma[ct] : 1.f, btt = T && ct < d && D.beta ? D.beta[ct] : 0.f;
-  const int64_t step = W == 1 ? (int64_t)gridDim.x * 4 : (int64_t)gridDim.x;
-  for (int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x; row < D.rows; row += step) {
+  const int64_t step = (int64_t)gridDim.x * R;
+  for (int64_t row = (int64_t)blockIdx.x * R + (L < 64 ? (int)threadIdx.x / L : W == 1 ? wave : 0); row < D.rows; row += step) {
     Raw8 xr[NV], rr[NV];
+    const bool whole = row + 2 < D.rows;       // the last chunk of a row as one load, its pads cleared afterwards
 #pragma unroll
-    for (int i = 0; i < NV; ++i) xr[i] = raw_load8<XF>((const char*)D.x + row * D.ldx * (XF ? 4 : 2), t0 + i * W * 512, d);
+    for (int i = 0; i < NV; ++i) xr[i] = raw_load8<XF>((const char*)D.x + row * D.ldx * (XF ? 4 : 2), t0 + i * W * 512, d, whole);
     if (RT) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) rr[i] = raw_load8<RT == 2>((const char*)D.res + row * D.ldr * (RT == 2 ? 4 : 2), t0 + i * W * 512, d);
+      for (int i = 0; i < NV; ++i) rr[i] = raw_load8<RT == 2>((const char*)D.res + row * D.ldr * (RT == 2 ? 4 : 2), t0 + i * W * 512, d, whole);
     }
     float vt = 0.f;
     if (T) {
@@ -93,6 +103,10 @@ __global__ __launch_bounds__(256) void addnorm_fwd_kernel(const vita_addnorm_fwd
 #pragma unroll
         for (int r = 0; r < 8; ++r) v[i][r] += t[r];
       }
+      if (t0 + i * W * 512 + 8 > d) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) if (t0 + i * W * 512 + r >= d) v[i][r] = 0.f;
+      }
 #pragma unroll
       for (int r = 0; r < 8; ++r) s += v[i][r];
     }
@@ -103,7 +117,7 @@ __global__ __launch_bounds__(256) void addnorm_fwd_kernel(const vita_addnorm_fwd
       if (T) store1((char*)D.sum + row * D.ldsum * (D.sum_dtype == VITA_DT_F32 ? 4 : 2), ct, D.ldsum, D.sum_dtype == VITA_DT_F32, vt);
     }
     if (D.kind == AN_LAYER) {
-      const float mu = (float)(row_sum<W>(s, red, turn, wave, lane) * inv_d);
+      const float mu = (float)(row_sum<W, L>(s, red, turn, wave, lane) * inv_d);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -124,7 +138,7 @@ __global__ __launch_bounds__(256) void addnorm_fwd_kernel(const vita_addnorm_fwd
     }
     // rstd as a pair of floats from 64 bits, n rounded once from its product: an error in the last bit of rstd would send ten times as
     // many values across the borders of the 8-bit codes as the roundings that are left
-    const double r = 1.0 / sqrt((double)row_sum<W>(q, red, turn, wave, lane) * inv_d + (double)D.eps);
+    const double r = 1.0 / sqrt((double)row_sum<W, L>(q, red, turn, wave, lane) * inv_d + (double)D.eps);
     const float rs = (float)r, rl = (float)(r - (double)rs);
     if (D.rstd && t0 == 0) D.rstd[row] = rs;
     const int dq = (d + 31) & ~31;
@@ -192,28 +206,35 @@ extern "C" int vita_addnorm_fwd(const vita_addnorm_fwd_desc* dp, void* stream) {
   VITA_REQUIRE(D.rows < (int64_t)0x7fffffff);
   const int rt = D.res ? (D.res_dtype == VITA_DT_F32 ? 2 : 1) : 0;
   const int al = (((uintptr_t)D.gamma | (uintptr_t)D.beta) & 15) == 0;
-  const auto blocks = [&](int w) { const int64_t n = w == 1 ? (D.rows + 3) / 4 : D.rows; return n < AN_FWD_MAXBLK ? n : AN_FWD_MAXBLK; };
-#define AN_LAUNCH(W, NV, T, XF, RT) \
-  hipLaunchKernelGGL((addnorm_fwd_kernel<W, NV, T, XF, RT>), dim3((unsigned)(blocks(W))), dim3(256), 0, (hipStream_t)stream, D, al)
-#define AN_TYPES(W, NV, T)                                                                                                                   \
+  const auto blocks = [&](int w, int m) {
+    const int64_t at_once = w > 1 ? 1 : m > AN_TAIL ? 256 / m : 4, n = (D.rows + at_once - 1) / at_once;
+    return n < AN_FWD_MAXBLK ? n : AN_FWD_MAXBLK;
+  };
+#define AN_LAUNCH(W, NV, M, XF, RT) \
+  hipLaunchKernelGGL((addnorm_fwd_kernel<W, NV, M, XF, RT>), dim3((unsigned)(blocks(W, M))), dim3(W == 1 ? 256 : 64 * W), 0, (hipStream_t)stream, D, al)
+#define AN_TYPES(W, NV, M)                                                                                                                   \
   do {                                                                                                                                       \
     if (D.x_dtype == VITA_DT_F32) {                                                                                                          \
-      if (rt == 0) AN_LAUNCH(W, NV, T, true, 0); else if (rt == 1) AN_LAUNCH(W, NV, T, true, 1); else AN_LAUNCH(W, NV, T, true, 2);         \
+      if (rt == 0) AN_LAUNCH(W, NV, M, true, 0); else if (rt == 1) AN_LAUNCH(W, NV, M, true, 1); else AN_LAUNCH(W, NV, M, true, 2);         \
     } else {                                                                                                                                 \
-      if (rt == 0) AN_LAUNCH(W, NV, T, false, 0); else if (rt == 1) AN_LAUNCH(W, NV, T, false, 1); else AN_LAUNCH(W, NV, T, false, 2);      \
+      if (rt == 0) AN_LAUNCH(W, NV, M, false, 0); else if (rt == 1) AN_LAUNCH(W, NV, M, false, 1); else AN_LAUNCH(W, NV, M, false, 2);      \
     }                                                                                                                                        \
   } while (0)
   // Few rows: four waves to a row shorten the way through one row, many rows: a wave to each saves the barriers.  One wave / four, us,
   // bf16 + fp32 residual, 600 columns: 1 row 3.7 / 3.0, 512 rows 5.3 / 4.8, 1024 5.8 / 6.0, 2048 7.0 / 8.7; 1025 columns: 3.8 / 3.2,
   // 5.6 / 5.2, 6.2 / 6.3, 8.3 / 9.7.  Above 1536 columns a wave would hold 4 chunks and more (64 registers of values): four waves, with
-  // one chunk a lane as far as that goes (2000 columns, 8192 rows: 34.0 us, with two chunks, half of them empty, 36.6).
-  if (width <= 512) AN_TYPES(1, 1, false);
-  else if (width <= 2048 && (D.rows <= AN_FEW_ROWS || width > 1536)) AN_TYPES(4, 1, false);
-  else if (width <= 1024) AN_TYPES(1, 2, false);
-  else if (width <= 1088) AN_TYPES(1, 2, true);
-  else if (width <= 1536) AN_TYPES(1, 3, false);
-  else if (width <= 4096) AN_TYPES(4, 2, false);
-  else AN_TYPES(4, 4, false);
+  // one chunk a lane as far as that goes (2000 columns, 8192 rows: 34.0 us, with two chunks, half of them empty, 36.6; from 2049 to
+  // 8192 columns more waves with one chunk each gain nothing, 119 us against 139 at 9000 x 5000).  Narrow rows share a wave: 46082 rows
+  // of 69 columns, 16 lanes each 11.2 us, 64 lanes 24.4; of 130 columns, 32 lanes 15.9 us, 64 lanes 24.6.
+  if (width <= 128) AN_TYPES(1, 1, 16);
+  else if (width <= 256) AN_TYPES(1, 1, 32);
+  else if (width <= 512) AN_TYPES(1, 1, AN_FULL);
+  else if (width <= 2048 && (D.rows <= AN_FEW_ROWS || width > 1536)) AN_TYPES(4, 1, AN_FULL);
+  else if (width <= 1024) AN_TYPES(1, 2, AN_FULL);
+  else if (width <= 1088) AN_TYPES(1, 2, AN_TAIL);
+  else if (width <= 1536) AN_TYPES(1, 3, AN_FULL);
+  else if (width <= 4096) AN_TYPES(4, 2, AN_FULL);
+  else AN_TYPES(4, 4, AN_FULL);
 #undef AN_TYPES
 #undef AN_LAUNCH
   VITA_CHECK_LAUNCH("vita_addnorm_fwd");
@@ -223,12 +244,14 @@ extern "C" int vita_addnorm_fwd(const vita_addnorm_fwd_desc* dp, void* stream) {
 // ---- backward: rows as above; every load of a row is in flight before its first sum, the values are taken from the raw registers
 // twice (to sum, to store) instead of being kept, and a lane's dgamma / dbeta sums stay in registers until one partial row per block
 #define AN_BWD_MAXBLK 768
-template <int W, int NV, bool T, int SRC, bool DYF>      // SRC: 0 8-bit rows, 1 bf16 sum, 2 fp32 sum
-__global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd_desc D, const int al) {
+template <int W, int NV, int M, int SRC, bool DYF>      // SRC: 0 8-bit rows, 1 bf16 sum, 2 fp32 sum
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, M == AN_TAIL ? 3 : 1) void addnorm_bwd_kernel(const vita_addnorm_bwd_desc D, const int al) {
+  constexpr bool T = M == AN_TAIL;
+  constexpr int L = M > AN_TAIL ? M : 64, R = W == 1 ? 256 / L : 1;      // as in the forward kernel
   __shared__ float red[2][2][W];
   __shared__ __attribute__((aligned(16))) float sums[W == 1 ? NV * 512 + 64 : 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int d = (int)D.d, t0 = (W == 1 ? lane : (int)threadIdx.x) * 8, nblk = gridDim.x;
+  const int d = (int)D.d, t0 = (W == 1 ? lane % L : (int)threadIdx.x) * 8, nblk = gridDim.x;
   const float inv_d = 1.f / (float)d;
   const bool dxf = D.dx_dtype == VITA_DT_F32;
   int turn = 0;
@@ -242,14 +265,15 @@ __global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd
   const int ct = NV * 512 + lane;                // the lane's column behind the chunks
   const float gt = T && ct < d && D.gamma ? D.gamma[ct] : 1.f;
   float agt = 0.f, abt = 0.f;
-  const int64_t step = W == 1 ? (int64_t)nblk * 4 : nblk;
-  for (int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x; row < D.rows; row += step) {
+  const int64_t step = (int64_t)nblk * R;
+  for (int64_t row = (int64_t)blockIdx.x * R + (L < 64 ? (int)threadIdx.x / L : W == 1 ? wave : 0); row < D.rows; row += step) {
     Raw8 dyr[NV], sr[NV], ir[NV];
     uint32_t byte[NV];
+    const bool whole = !T && row + 2 < D.rows; // the last chunk of a row as one load (pieces cost a wait in front of the next operand's)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = t0 + i * W * 512;
-      dyr[i] = raw_load8<DYF>((const char*)D.dy + row * D.lddy * (DYF ? 4 : 2), c, d);
+      dyr[i] = raw_load8<DYF>((const char*)D.dy + row * D.lddy * (DYF ? 4 : 2), c, d, whole);
       if (SRC == 0) {
         sr[i].a = u32x4{0, 0, 0, 0};
         byte[i] = 127;
@@ -259,16 +283,16 @@ __global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd
           byte[i] = ((const uint8_t*)D.scale)[row * D.lds + (c >> 5)];
         }
       } else {
-        sr[i] = raw_load8<SRC == 2>((const char*)D.src + row * D.ldx * (SRC == 2 ? 4 : 2), c, d);
+        sr[i] = raw_load8<SRC == 2>((const char*)D.src + row * D.ldx * (SRC == 2 ? 4 : 2), c, d, whole);
       }
     }
     if (D.dx_in) {
       if (dxf) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) ir[i] = raw_load8<true>((const float*)D.dx_in + row * D.lddx_in, t0 + i * W * 512, d);
+        for (int i = 0; i < NV; ++i) ir[i] = raw_load8<true>((const float*)D.dx_in + row * D.lddx_in, t0 + i * W * 512, d, whole);
       } else {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) ir[i] = raw_load8<false>((const uint16_t*)D.dx_in + row * D.lddx_in, t0 + i * W * 512, d);
+        for (int i = 0; i < NV; ++i) ir[i] = raw_load8<false>((const uint16_t*)D.dx_in + row * D.lddx_in, t0 + i * W * 512, d, whole);
       }
     }
     const float rs = D.rstd[row], mu = SRC != 0 && D.mean ? D.mean[row] : 0.f;
@@ -292,9 +316,9 @@ __global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd
         for (int r = 0; r < 8; ++r) n[r] = (n[r] - mu) * rs;
       }
       const int c = t0 + i * W * 512;
-      if (c + 8 > d) {                                 // dy is zero there already
+      if (c + 8 > d) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) if (c + r >= d) n[r] = 0.f;
+        for (int r = 0; r < 8; ++r) if (c + r >= d) { n[r] = 0.f; if (!T) dy[r] = 0.f; }
       }
     };
     float s1 = 0.f, s2 = 0.f;
@@ -317,7 +341,7 @@ __global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd
         s2 = __builtin_fmaf(h, n[r], s2);
       }
     }
-    row_sum2<W>(s1, s2, red, turn, wave, lane);
+    row_sum2<W, L>(s1, s2, red, turn, wave, lane);
     // the values once more from the raw registers (the empty asm keeps the compiler from holding them over the sum: 16 NV registers)
 #pragma unroll
     for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(dyr[i].a), "+v"(sr[i].a));
@@ -349,6 +373,12 @@ __global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd
     }
   }
   if (!D.partial) return;
+  if (L < 64) {                         // the wave's rows first
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int o = L; o < 64; o <<= 1) { ag[0][r] += __shfl_xor(ag[0][r], o, 64); ab[0][r] += __shfl_xor(ab[0][r], o, 64); }
+  }
   float* pg = D.partial + (int64_t)blockIdx.x * d;
   float* pb = D.partial + ((int64_t)nblk + blockIdx.x) * d;
 #pragma unroll
@@ -357,7 +387,7 @@ __global__ __launch_bounds__(256) void addnorm_bwd_kernel(const vita_addnorm_bwd
     if (W == 1) {                       // the block's four waves one after another, through LDS
       for (int w = 0; w < 4; ++w) {
         __syncthreads();
-        if (wave == w) {
+        if (wave == w && lane < L) {
 #pragma unroll
           for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -414,8 +444,9 @@ __global__ __launch_bounds__(1024) void addnorm_reduce_kernel(const float* __res
 }
 
 extern "C" int64_t vita_addnorm_bwd_nblk(int64_t rows, int64_t d) {
-  const int64_t n = d <= 1536 ? (rows + 7) / 8 : (rows + 1) / 2;
-  const int64_t most = d > 1088 && d <= 1536 ? AN_BWD_MAXBLK * 2 / 3 : AN_BWD_MAXBLK;      // as many blocks as are resident: 2 or 3 a CU
+  // two rows at least for a wave (for a block of several waves to a row), and no more blocks than are resident: 1 to 3 a CU
+  const int64_t n = d <= 128 ? (rows + 31) / 32 : d <= 256 ? (rows + 15) / 16 : d <= 1536 ? (rows + 7) / 8 : (rows + 1) / 2;
+  const int64_t most = d > 4096 ? AN_BWD_MAXBLK / 3 : d > 2048 || (d > 1088 && d <= 1536) ? AN_BWD_MAXBLK * 2 / 3 : AN_BWD_MAXBLK;
   return n < most ? n : most;
 }
 
@@ -443,25 +474,31 @@ extern "C" int vita_addnorm_bwd(const vita_addnorm_bwd_desc* dp, void* stream) {
   const int nblk = (int)vita_addnorm_bwd_nblk(D.rows, D.d);
   const int al = ((uintptr_t)D.gamma & 15) == 0;
   const int src = D.q ? 0 : (D.src_dtype == VITA_DT_F32 ? 2 : 1);
-#define AN_LAUNCH(W, NV, T, SRC, DYF) \
-  hipLaunchKernelGGL((addnorm_bwd_kernel<W, NV, T, SRC, DYF>), dim3(nblk), dim3(256), 0, (hipStream_t)stream, D, al)
-#define AN_TYPES(W, NV, T)                                                                                                                   \
+#define AN_LAUNCH(W, NV, M, SRC, DYF) \
+  hipLaunchKernelGGL((addnorm_bwd_kernel<W, NV, M, SRC, DYF>), dim3(nblk), dim3(W == 1 ? 256 : 64 * W), 0, (hipStream_t)stream, D, al)
+#define AN_TYPES(W, NV, M)                                                                                                                   \
   do {                                                                                                                                       \
     if (D.dy_dtype == VITA_DT_F32) {                                                                                                         \
-      if (src == 0) AN_LAUNCH(W, NV, T, 0, true); else if (src == 1) AN_LAUNCH(W, NV, T, 1, true); else AN_LAUNCH(W, NV, T, 2, true);       \
+      if (src == 0) AN_LAUNCH(W, NV, M, 0, true); else if (src == 1) AN_LAUNCH(W, NV, M, 1, true); else AN_LAUNCH(W, NV, M, 2, true);       \
     } else {                                                                                                                                 \
-      if (src == 0) AN_LAUNCH(W, NV, T, 0, false); else if (src == 1) AN_LAUNCH(W, NV, T, 1, false); else AN_LAUNCH(W, NV, T, 2, false);    \
+      if (src == 0) AN_LAUNCH(W, NV, M, 0, false); else if (src == 1) AN_LAUNCH(W, NV, M, 1, false); else AN_LAUNCH(W, NV, M, 2, false);    \
     }                                                                                                                                        \
   } while (0)
-  // One wave a row up to 1536 columns, four beyond, us from 8 bits, fp32 dx_in and dx: 1025 columns, 30000 rows: 70 with one, 121 with
-  // four; 2000 columns: 140 with four of one chunk, 158 of two (half of them empty).
-  if (width <= 512) AN_TYPES(1, 1, false);
-  else if (width <= 1024) AN_TYPES(1, 2, false);
-  else if (width <= 1088) AN_TYPES(1, 2, true);
-  else if (width <= 1536) AN_TYPES(1, 3, false);
-  else if (width <= 2048) AN_TYPES(4, 1, false);
-  else if (width <= 4096) AN_TYPES(4, 2, false);
-  else AN_TYPES(4, 4, false);
+  // One wave a row up to 1536 columns (30000 x 1025 from 8 bits, fp32 dx_in and dx: 70 us, with four waves 121), beyond as many waves as
+  // hold the row with one chunk a lane, since a chunk costs some 50 registers here: 20000 x 2000 140 us with four waves, 158 with two chunks
+  // a lane; fp32 dy, bf16 dx_in and dx: 17918 x 2636 102 with six, 135 with eight and 205 with four of two chunks; 9000 x 5000 96
+  // with twelve, 115 with sixteen, 209 with four of four.  Narrow rows as in the forward pass: 46082 x 69 11.4 against 26.4 us.
+  if (width <= 128) AN_TYPES(1, 1, 16);
+  else if (width <= 256) AN_TYPES(1, 1, 32);
+  else if (width <= 512) AN_TYPES(1, 1, AN_FULL);
+  else if (width <= 1024) AN_TYPES(1, 2, AN_FULL);
+  else if (width <= 1088) AN_TYPES(1, 2, AN_TAIL);
+  else if (width <= 1536) AN_TYPES(1, 3, AN_FULL);
+  else if (width <= 2048) AN_TYPES(4, 1, AN_FULL);
+  else if (width <= 6 * 512) AN_TYPES(6, 1, AN_FULL);
+  else if (width <= 4096) AN_TYPES(8, 1, AN_FULL);
+  else if (width <= 6144) AN_TYPES(12, 1, AN_FULL);
+  else AN_TYPES(16, 1, AN_FULL);
 #undef AN_TYPES
 #undef AN_LAUNCH
   VITA_CHECK_LAUNCH("vita_addnorm_bwd");
