@@ -459,6 +459,20 @@ def test_offsets_beyond_32_bits(ops):
     assert torch.equal(dx[-5:], ops.addnorm_bwd(tail, few.act, few.rstd, dx_dtype=BF16, want_dgamma=False)[0])
 
 
+@pytest.mark.parametrize("k,m,n", [(46082, 20, 20), (46082, 300, 200), (46082, 300, 300), (69262, 8, 6625)])
+def test_wgrad_of_many_parts(ops, k, m, n):
+    """Long sums in 32 and more parts to an element, joined by one lane or by eight; the last case deals out a line of short pieces.
+    The 64-bit product is taken on the device."""
+    g = torch.Generator(device="cuda").manual_seed(k + m)
+    x = torch.randn(k, -(-n // 8) * 8, device="cuda", generator=g).to(BF16)[:, :n]
+    dy = torch.randn(k, -(-m // 8) * 8, device="cuda", generator=g).to(BF16)[:, :m]
+    a = ops.act8_pack(x)
+    dw = ops.act8_wgrad(dy, a)
+    v, d = ops.act8_unpack(a)[:, :n].double(), dy.double().t().contiguous()
+    close(dw, (d @ v).cpu(), ((8 * k ** 0.5 + 8) * U * (d.abs() @ v.abs())).cpu() + 1e-30)
+    assert torch.equal(dw, ops.act8_wgrad(dy, a))
+
+
 @pytest.mark.parametrize("which", ["dy", "codes"])
 def test_wgrad_over_more_than_2_gib(ops, which):
     """Rows 2 MiB (dy) or 1 MiB (codes) apart: the sum needs more than one call of the kernel; pads of dy hold NaN."""

@@ -40,6 +40,7 @@ struct Wgrad8Params {
   int tiles_m, tiles_n, kt;      // kt = K-tiles of one tile
   int whole;                     // tiles [0, whole) are never cut: whole / W8_WGS per workgroup
   int cut, cut_tiles;            // tiles [whole, whole + cut_tiles) in `cut` parts each, cut_tiles * cut <= W8_WGS
+  int cut_kt, cut_more;          // K-tiles of a part; one more in the first cut_more of them
   int piece, pieces;             // the K-tiles of the other tiles, in one line, dealt out in pieces of `piece`
   int accumulate;
 };
@@ -54,7 +55,7 @@ __device__ __forceinline__ int64_t w8_cut_slot(const Wgrad8Params& P, int tile, 
 __device__ __forceinline__ int64_t w8_piece_slot(const Wgrad8Params& P, int piece, int second) {
   return (int64_t)P.cut_tiles * P.cut + 2 * piece + second;
 }
-__device__ __forceinline__ int w8_cut_begin(const Wgrad8Params& P, int part) { return (int)((int64_t)P.kt * part / P.cut); }
+__device__ __forceinline__ int w8_cut_begin(const Wgrad8Params& P, int part) { return part * P.cut_kt + (part < P.cut_more ? part : P.cut_more); }
 
 // 4 neighbouring columns of a row of dw, `left` of them inside; rows start on any 4-byte boundary, which 16-byte stores take too
 __device__ __forceinline__ void w8_put(const Wgrad8Params& P, float* o, f32x4 v, int64_t left) {
@@ -303,30 +304,37 @@ __global__ __launch_bounds__(G2_THREADS, 2) void act8_wgrad_kernel(const Wgrad8P
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < NFW; ++j)
-          if (j < nfw) *reinterpret_cast<f32x4*>(o + (rl + 16 * i) * (NF * 16) + cl + 16 * j) = acc[i][j];
+        for (int j = 0; j < NFW; ++j)          // fragments that hold something of dw
+          if (j < nfw && m0 + wm * 64 + 16 * i < P.m && n0 + (wn * NFW + j) * 16 < P.n) *reinterpret_cast<f32x4*>(o + (rl + 16 * i) * (NF * 16) + cl + 16 * j) = acc[i][j];
     }
   }
 }
 
-// s + p[0] + p[step] + ... + p[(n - 1) step], eight loads in flight
-__device__ __forceinline__ f32x4 w8_sum_parts(const float* p, int n, int64_t step, f32x4 s) {
-  for (int i = 0; i < n; i += 8) {
+// p[sub] + p[sub + S] + ... of n parts `step` floats apart, eight loads in flight; then over the S neighbouring lanes (sub = 0 .. S - 1)
+template <int S>
+__device__ __forceinline__ f32x4 w8_sum_parts(const float* p, int n, int64_t step, int sub) {
+  f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = sub; i < n; i += 8 * S) {
     f32x4 t[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      if (i + u < n) t[u] = *reinterpret_cast<const f32x4*>(p + (i + u) * step);
+      if (i + u * S < n) t[u] = *reinterpret_cast<const f32x4*>(p + (i + u * S) * step);
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      if (i + u < n) s += t[u];
+      if (i + u * S < n) s += t[u];
   }
+#pragma unroll
+  for (int o = 1; o < S; o <<= 1)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[r] += __shfl_xor(s[r], o, 64);
   return s;
 }
-// adds the parts of each tile that was cut, in their order: grid (tiles behind the whole ones, quads of a tile / 256); a thread owns
-// 4 neighbouring columns of a row
+// adds the parts of each tile that was cut, always in the same order: grid (tiles behind the whole ones, quads of a tile * S / 256); S
+// neighbouring lanes own 4 neighbouring columns of a row
+template <int S>
 __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const Wgrad8Params P, const int width) {
   const int tile = P.whole + blockIdx.x;
-  const int quad = blockIdx.y * 256 + threadIdx.x;
+  const int at = blockIdx.y * 256 + threadIdx.x, quad = at / S, sub = at % S;
   const int per_row = width / 4;
   const int rl = quad / per_row, cl = (quad - rl * per_row) * 4;
   int tm, tn;
@@ -335,22 +343,25 @@ __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const Wgrad8Params
   if (rl >= 256 || row >= P.m || col >= P.n) return;
   const int64_t slot_floats = 256 * (int64_t)width;
   const float* p = P.ws + (int64_t)rl * width + cl;
-  f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 s;
   if (blockIdx.x < (unsigned)P.cut_tiles) {
     if (P.cut == 1) return;                              // written already
-    s = w8_sum_parts(p + w8_cut_slot(P, tile, 0) * slot_floats, P.cut, slot_floats, s);
+    s = w8_sum_parts<S>(p + w8_cut_slot(P, tile, 0) * slot_floats, P.cut, slot_floats, sub);
   } else {
     const int64_t t0 = (int64_t)(blockIdx.x - P.cut_tiles) * P.kt, t1 = t0 + P.kt;
     const int w0 = (int)(t0 / P.piece), w1 = (int)((t1 + P.piece - 1) / P.piece);
-    if ((int64_t)w0 * P.piece < t0) s = *reinterpret_cast<const f32x4*>(p + w8_piece_slot(P, w0, 1) * slot_floats);
-    else s = *reinterpret_cast<const f32x4*>(p + w8_piece_slot(P, w0, 0) * slot_floats);
-    s = w8_sum_parts(p + w8_piece_slot(P, w0 + 1, 0) * slot_floats, w1 - w0 - 1, 2 * slot_floats, s);
+    // the first part may be the second half of its piece
+    const f32x4 first = *reinterpret_cast<const f32x4*>(p + w8_piece_slot(P, w0, (int64_t)w0 * P.piece < t0) * slot_floats);
+    s = first + w8_sum_parts<S>(p + w8_piece_slot(P, w0 + 1, 0) * slot_floats, w1 - w0 - 1, 2 * slot_floats, sub);
   }
-  w8_put(P, P.dw + row * P.lddw + col, s, P.n - col);
+  if (sub == 0) w8_put(P, P.dw + row * P.lddw + col, s, P.n - col);
 }
 
 // ---- host
 struct Wgrad8Plan { int nf, grid, whole, cut, cut_tiles, piece, pieces; int64_t slots; };
+// Many parts and few elements: eight lanes share the parts of an element.  One lane / eight, us: 46082 tokens, 20 x 20 in 128 parts 14.0 /
+// 4.0, 200 x 300 9.6 / 6.0, 64 x 1025 7.3 / 5.8, 300 x 300 9.0 / 9.6 (shorter runs of memory to a load), 600 x 600 8.6 / 11.0.
+static bool w8_deep(int64_t elements, int64_t cut, int64_t line_depth) { return elements <= 80000 && (cut > 16 || line_depth > 16); }
 // The cheapest of the tile widths and cuts, in microseconds of the longest workgroup: K-tiles (measured 1.30 us at 128 columns, 1.38
 // at 208, 1.53 at 256), start and end of each part, and the parts' way to the workspace and back over the whole chip
 // (256 x 16 nf floats written and read at 5 TB/s) with the join's launch and the depth of its sums.
@@ -358,6 +369,7 @@ static Wgrad8Plan w8_plan(int64_t m, int64_t n, int64_t k) {
   const int64_t tm = (m + 255) / 256, kt = (k + G2_BK - 1) / G2_BK;
   Wgrad8Plan best = {};
   double cost = -1;
+  const double filled = (double)m / (tm * 256);          // rows of the tiles that are written
   const int cand[3] = {8, 13, 16};
   for (int c = 0; c < 3; ++c) {
     const int nf = cand[c];
@@ -372,10 +384,11 @@ static Wgrad8Plan w8_plan(int64_t m, int64_t n, int64_t k) {
       const int64_t pieces = (line + piece - 1) / piece;
       const int64_t slots = (cut > 1 ? ct * cut : 0) + (line ? pieces + (left - ct) : 0);
       const double kt_us = nf == 8 ? 1.30 : nf == 13 ? 1.38 : 1.53;
-      const double longest = (double)(whole / W8_WGS) * (kt * kt_us + 4) + (left ? (kt + cut - 1) / cut * kt_us + 4 : 0) +
-                             (line ? piece * kt_us + 4 : 0);
-      const double depth = line ? (double)kt / piece : (double)cut;
-      const double x = longest + (slots ? 0.0065 * nf * slots + 4 + 0.1 * depth : 0);
+      const double longest = (double)(whole / W8_WGS) * (kt * kt_us + 5) + (left ? (kt + cut - 1) / cut * kt_us + 5 : 0) +
+                             (line ? piece * kt_us + 5 : 0);
+      double depth = line ? (double)kt / piece : (double)cut;
+      if (w8_deep(m * n, cut, line ? kt / piece : 0)) depth /= 8;
+      const double x = longest + (slots ? 0.0065 * nf * slots * filled + 4 + 0.1 * depth : 0);
       if (cost < 0 || x < cost) {
         cost = x;
         const int64_t busy = whole ? W8_WGS : (ct * cut > pieces ? ct * cut : pieces);
@@ -400,7 +413,11 @@ static int w8_launch(const Wgrad8Params& P, int grid, bool join, hipStream_t s) 
   hipLaunchKernelGGL(act8_wgrad_kernel<NF>, dim3((unsigned)grid), dim3(G2_THREADS), lds, s, P);
   VITA_CHECK_LAUNCH("vita_act8_wgrad");
   if (join) {
-    hipLaunchKernelGGL(act8_wgrad_join_kernel, dim3((unsigned)(P.tiles_m * P.tiles_n - P.whole), 4 * NF), dim3(256), 0, s, P, NF * 16);
+    const unsigned tiles = (unsigned)(P.tiles_m * P.tiles_n - P.whole);
+    if (w8_deep(P.m * P.n, P.cut, P.pieces ? P.kt / P.piece : 0))
+      hipLaunchKernelGGL(act8_wgrad_join_kernel<8>, dim3(tiles, 32 * NF), dim3(256), 0, s, P, NF * 16);
+    else
+      hipLaunchKernelGGL(act8_wgrad_join_kernel<1>, dim3(tiles, 4 * NF), dim3(256), 0, s, P, NF * 16);
     VITA_CHECK_LAUNCH("vita_act8_wgrad_join");
   }
   return VITA_OK;
@@ -421,6 +438,7 @@ extern "C" int vita_act8_wgrad(const void* dy, int64_t lddy, const void* q, int6
   const int64_t tiles_m = (m + 255) / 256, tiles_n = (n + plan.nf * 16 - 1) / (plan.nf * 16), kt = (k + G2_BK - 1) / G2_BK;
   VITA_REQUIRE(tiles_m * tiles_n < ((int64_t)1 << 30));
   P.tiles_m = (int)tiles_m; P.tiles_n = (int)tiles_n; P.kt = (int)kt;
+  P.cut_kt = P.kt / plan.cut; P.cut_more = P.kt % plan.cut;
   P.whole = plan.whole; P.cut = plan.cut; P.cut_tiles = plan.cut_tiles; P.piece = plan.piece; P.pieces = plan.pieces;
   P.accumulate = accumulate;
   // 32-bit offsets inside a part's tokens (a part is at most kt K-tiles long, and is read up to 3 K-tiles past its end)
