@@ -16,8 +16,8 @@
 //   * a part of a tile goes to the workspace as fp32; a second kernel adds a tile's parts in their order.  One writer per
 //     element, no atomics: the same bits on every call.
 //
-// Measured (MI355X): 3776 tokens, 1025 x 4100: 42 + 13 us (join), 750 TFLOP/s without the join; 13826 tokens, 1025 x 3075: 109 + 13 us,
-// 800 TFLOP/s; the bf16 kernel of gemm256.hip with atomics takes 85 and 131 us for the same shapes, without the pass that restores its
+// Measured (MI355X): 3776 tokens, 1025 x 4100: 42 + 13 us (join), 750 TFLOP/s without the join; 13826 tokens, 1025 x 3075: 100 to 109 + 13
+// us, 800 to 870 TFLOP/s; the bf16 kernel of gemm256.hip with atomics takes 85 and 131 us for the same shapes, without the pass that restores its
 // operand.  Bound by what one wave after another can issue: without the conversions 98 us of the 109 are left, without the DMA of dy
 // 96, without either 85 (matrix instructions, fragment reads, barriers); without the loads of the codes 109.  With all waves in step and
 // the conversions in one piece behind the barrier the two shapes take 43 and 114 to 122 us; with four waves of twice the rows 124; when
