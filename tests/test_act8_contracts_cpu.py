@@ -1,0 +1,32 @@
+"""What the modules around the 8-bit checkpoints and residual norms decide before any kernel runs, checked without a GPU."""
+import pytest
+import torch
+from torch import nn
+
+
+@pytest.fixture(scope="module")
+def V():
+    import vita_amd.nn as v
+    return v
+
+
+class PlainNorm(nn.Module):
+    """A layer norm that is no nn.LayerNorm: weight, bias, eps and normalized_shape are all that the kernels ask of one."""
+
+    def __init__(self, dim, eps=1e-5):
+        super().__init__()
+        self.weight, self.bias, self.eps, self.normalized_shape = nn.Parameter(torch.ones(dim)), nn.Parameter(torch.zeros(dim)), eps, (dim,)
+
+
+@pytest.mark.parametrize("first,second,bits,want", [
+    (nn.LayerNorm, nn.LayerNorm, 16, "_BlockFn"), (PlainNorm, PlainNorm, 16, "_BlockFn"), (PlainNorm, nn.LayerNorm, 16, "_BlockFn"),
+    (nn.RMSNorm, nn.LayerNorm, 16, "_BlockActFn"), (nn.LayerNorm, nn.RMSNorm, 16, "_BlockActFn"), (nn.RMSNorm, nn.RMSNorm, 16, "_BlockActFn"),
+    (nn.LayerNorm, nn.LayerNorm, 8, "_BlockActFn"), (nn.LayerNorm, nn.RMSNorm, 8, "_BlockActFn")])
+def test_both_norms_choose_the_function_of_a_block(V, monkeypatch, first, second, bits, want):
+    seen = []
+    for name in ("_BlockFn", "_BlockActFn"):
+        monkeypatch.setattr(getattr(V, name), "apply", lambda *a, name=name: seen.append(name))
+    b = V.Block(16, 2, 4.0, qkv_bias=True, saved_bits=bits)
+    b.norm1, b.norm2 = first(16), second(16)
+    b.forward_padded(torch.zeros(1, 2, 64))
+    assert seen == [want]

@@ -1,0 +1,81 @@
+"""What the entry points of the 8-bit checkpoints and residual norms promise beside their formulas: Blocks whose two norms differ,
+second derivatives, capture, buffers that serve as input and output, sums added to what a buffer holds, matrices that end with
+their last element."""
+import pytest
+import torch
+from torch import nn
+
+import act8_reference as R
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+U = 2.0 ** -24
+BF16_TOL, STORED = 2e-2, 2.0 ** -4          # roundings of bf16 products; half an e4m3 step
+
+
+@pytest.fixture(scope="module")
+def V():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    import vita_amd.nn as v
+    return v
+
+
+def rel(a, b):
+    a, b = a.detach().cpu().double(), b.detach().cpu().double()
+    return ((a - b).norm() / b.norm().clamp_min(1e-30)).item()
+
+
+# ------------------------------------------------------------------------------------------------ norms of two kinds
+def mixed_block(V, D, H, first, second, bits):
+    torch.manual_seed(D)
+    b = V.Block(D, H, 4.0, qkv_bias=True, norm_layer=first, saved_bits=bits)
+    b.norm2 = second(D, eps=1e-3)                      # another eps too
+    with torch.no_grad():
+        for n, p in b.named_parameters():
+            if "norm" in n:
+                p.copy_((1.0 if "weight" in n else 0.0) + 0.5 * torch.randn_like(p))
+            elif p.dim() == 1:
+                p.copy_(0.1 * torch.randn_like(p))
+    return b.cuda()
+
+
+def plain_block(P, x, norms, H):
+    """The Block in float64: norms = (module class, eps) of norm1 and norm2."""
+    B, N, D = x.shape
+
+    def norm(t, k):
+        cls, eps = norms[k - 1]
+        if cls is nn.LayerNorm:
+            t = t - t.mean(-1, keepdim=True)
+        t = t / torch.sqrt(t.square().mean(-1, keepdim=True) + eps) * P[f"norm{k}.weight"]
+        return t + P[f"norm{k}.bias"] if cls is nn.LayerNorm else t
+
+    qkv = (norm(x, 1) @ P["attn.qkv.weight"].t() + P["attn.qkv.bias"]).view(B, N, 3, H, D // H).permute(2, 0, 3, 1, 4)
+    o = ((qkv[0] @ qkv[1].transpose(-1, -2)) * (D // H) ** -0.5).softmax(-1) @ qkv[2]
+    x = x + o.transpose(1, 2).reshape(B, N, D) @ P["attn.proj.weight"].t() + P["attn.proj.bias"]
+    z = norm(x, 2) @ P["mlp.fc1.weight"].t() + P["mlp.fc1.bias"]
+    return x + R.gelu(z)[0] @ P["mlp.fc2.weight"].t() + P["mlp.fc2.bias"]
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("first,second", [(nn.RMSNorm, nn.LayerNorm), (nn.LayerNorm, nn.RMSNorm)])
+def test_block_whose_norms_differ(V, first, second, bits):
+    """Each norm is its own kind, forward and backward.  8 bits: the stored factors add half an e4m3 step to the gradients."""
+    D, H, B, N = 129, 3, 2, 50
+    blk = mixed_block(V, D, H, first, second, bits)
+    g = torch.Generator().manual_seed(1)
+    x = (torch.randn(B, N, D, generator=g) + 1.0).cuda().requires_grad_()      # a mean that only LayerNorm takes away
+    dy = torch.randn(B, N, D, generator=g).cuda()
+    y = blk(x)
+    y.backward(dy)
+    P = {n: p.detach().cpu().double().requires_grad_() for n, p in blk.named_parameters()}
+    xr = x.detach().cpu().double().requires_grad_()
+    eps1 = torch.finfo(F32).eps if first is nn.RMSNorm else 1e-5
+    yr = plain_block(P, xr, ((first, eps1), (second, 1e-3)), H)
+    yr.backward(dy.cpu().double())
+    tol = BF16_TOL if bits == 16 else 2 * BF16_TOL + STORED
+    assert rel(y, yr) < BF16_TOL
+    assert rel(x.grad, xr.grad) < tol
+    for n, p in blk.named_parameters():
+        assert rel(p.grad, P[n].grad) < tol, n

@@ -515,7 +515,7 @@ class _BlockFn(torch.autograd.Function):
 
 
 def norm_kind(ln):
-    """"layer" or "rms" of a Block's norm module."""
+    """"layer" or "rms" of a Block's norm module; the two norms of a Block need not be of one kind."""
     return "rms" if isinstance(ln, nn.RMSNorm) else "layer"
 
 
@@ -536,12 +536,12 @@ def norm_grad_targets(ln, need_w, need_b):
     return (gw, None) if gw is not None else None
 
 
-def norm_bwd_padded(dy, src, rstd, ln, D, Dp, need_w, need_b, dx_in=None):
-    """Gradient of a norm on the padded stream from its 8-bit rows or (rms) its kept input: (dx fp32 [M, Dp], bf16 copy, dgamma, dbeta),
-    the two sums in place where the parameters allow it (None is returned for them then)."""
+def norm_bwd_padded(dy, src, rstd, ln, D, Dp, need_w, need_b, mean=None, dx_in=None):
+    """Gradient of a norm on the padded stream from its 8-bit rows or its kept input (then with mean for a LayerNorm): (dx fp32 [M, Dp],
+    bf16 copy, dgamma, dbeta), the two sums in place where the parameters allow it (None is returned for them then)."""
     acc = norm_grad_targets(ln, need_w, need_b)
     (dx, dxb), dw, db = ops.addnorm_bwd(dy[:, :D], src if isinstance(src, ops.Act8) else src[:, :D], rstd, ln.weight, kind=norm_kind(ln),
-                                        dx_in=None if dx_in is None else dx_in[:, :D], lddx=Dp, want_bf16=True,
+                                        mean=mean, dx_in=None if dx_in is None else dx_in[:, :D], lddx=Dp, want_bf16=True,
                                         want_dgamma=need_w, want_dbeta=need_b and _norm_bias(ln) is not None, acc=acc)
     if acc is not None:
         grad_done(ln.weight)
@@ -578,15 +578,14 @@ class _BlockActFn(torch.autograd.Function):
         sh = blk.shadows()
         x = xp.reshape(M, Dp)
         pack = "normed" if blk.saved_bits == 8 else None
-        kind, eps = norm_kind(blk.norm1), norm_eps(blk.norm1)
-        a1 = ops.addnorm_fwd(x[:, :D], n1w, n1b, kind=kind, eps=eps, pack=pack, ldy=Dp)
+        a1 = ops.addnorm_fwd(x[:, :D], n1w, n1b, kind=norm_kind(blk.norm1), eps=norm_eps(blk.norm1), pack=pack, ldy=Dp)
         qkv = torch.empty(M, dm.QKV, dtype=torch.bfloat16, device=x.device)
         ops.gemm(a1.y, sh["qkv_w"], qkv, M, dm.QKV, Dp, Dp, Dp, dm.QKV, bias=sh["qkv_b"], flops=6.0 * M * D * D)
         o, att_saved = attention_fwd(qkv, B, N, dm, DEFAULT_FLASH if blk.use_flash is None else blk.use_flash)
         x1 = torch.empty(M, Dp, dtype=torch.float32, device=x.device)
         ops.gemm(o, sh["proj_w"], x1, M, Dp, dm.AO, dm.AO, dm.AO, Dp, bias=sh["proj_b"], epilogue=ops.EPI_RESIDUAL,
                  aux_in=x, ld_aux=Dp, flops=2.0 * M * D * D)
-        a2 = ops.addnorm_fwd(x1[:, :D], n2w, n2b, kind=kind, eps=norm_eps(blk.norm2), pack=pack, ldy=Dp)
+        a2 = ops.addnorm_fwd(x1[:, :D], n2w, n2b, kind=norm_kind(blk.norm2), eps=norm_eps(blk.norm2), pack=pack, ldy=Dp)
         if pack:
             z = torch.empty(M, dm.Hp, dtype=torch.bfloat16, device=x.device)
             ops.gemm(a2.y, sh["fc1_w"], z, M, dm.Hp, Dp, Dp, Dp, dm.Hp, bias=sh["fc1_b"], flops=2.0 * M * D * dm.hidden)
@@ -605,7 +604,7 @@ class _BlockActFn(torch.autograd.Function):
             ctx.save_for_backward(a1.act.q, a1.act.scale, a1.rstd, qkv, o, a2.act.q, a2.act.scale, a2.rstd, z8.q, z8.scale,
                                   n1w, n1b, n2w, n2b, att_saved[1])
         else:
-            ctx.save_for_backward(x, a1.rstd, a1.y, qkv, o, x1, a2.rstd, a2.y, u, g, n1w, n1b, n2w, n2b, att_saved[1])
+            ctx.save_for_backward(x, a1.rstd, a1.y, qkv, o, x1, a2.rstd, a2.y, u, g, n1w, n1b, n2w, n2b, att_saved[1], a1.mean, a2.mean)
         return x2.view(B, N, Dp)
 
     @staticmethod
@@ -616,7 +615,8 @@ class _BlockActFn(torch.autograd.Function):
         B, N = ctx.shape
         M, Dp, D = B * N, dm.Dp, dm.D
         saved = ctx.saved_tensors
-        n1w, n1b, n2w, n2b, att_t = saved[10:]
+        n1w, n1b, n2w, n2b, att_t = saved[10:15]
+        mean1, mean2 = (None, None) if ctx.bits == 8 else saved[15:]         # of a LayerNorm whose input was kept
         if ctx.bits == 8:
             q1, s1, rstd1, qkv, o, q2, s2, rstd2, qz, sz = saved[:10]
             src1, src2, z8 = ops.Act8(q1, s1, D), ops.Act8(q2, s2, D), ops.Act8(qz, sz, dm.hidden)
@@ -646,7 +646,7 @@ class _BlockActFn(torch.autograd.Function):
         d_fc1b = side(bgrad, du, dm.Hp, M, dm.hidden, param=mlp.fc1.bias) if need[11] else None
         dln2 = torch.empty(M, Dp, dtype=torch.bfloat16, device=dev)
         ops.gemm(du, sh["fc1_w"], dln2, M, Dp, dm.Hp, dm.Hp, Dp, Dp, b_layout=1, flops=2.0 * M * D * dm.hidden)
-        dx1, dx1b, d_n2w, d_n2b = norm_bwd_padded(dln2, src2, rstd2, blk.norm2, D, Dp, need[8], need[9], dx_in=dx2)
+        dx1, dx1b, d_n2w, d_n2b = norm_bwd_padded(dln2, src2, rstd2, blk.norm2, D, Dp, need[8], need[9], mean2, dx_in=dx2)
         d_projw = side(wgrad, dx1b, Dp, o, dm.AO, D, D, M, col_seg=(dm.hdp, dm.hd), n_phys=dm.AO, param=a.proj.weight) \
             if need[6] else None
         d_projb = side(bgrad, dx1b, Dp, M, D, param=a.proj.bias) if need[7] else None
@@ -662,7 +662,7 @@ class _BlockActFn(torch.autograd.Function):
             d_qkvb = side(lambda: ops.unpack_vec(ops.colsum(dqkv, dm.QKV, M, dm.QKV), 3 * D, seg=(dm.hdp, dm.hd)))
         dln1 = torch.empty(M, Dp, dtype=torch.bfloat16, device=dev)
         ops.gemm(dqkv, sh["qkv_w"], dln1, M, Dp, dm.QKV, dm.QKV, Dp, Dp, b_layout=1, flops=6.0 * M * D * D)
-        dx, dxb, d_n1w, d_n1b = norm_bwd_padded(dln1, src1, rstd1, blk.norm1, D, Dp, need[2], need[3], dx_in=dx1)
+        dx, dxb, d_n1w, d_n1b = norm_bwd_padded(dln1, src1, rstd1, blk.norm1, D, Dp, need[2], need[3], mean1, dx_in=dx1)
         side.join()
         return (with_bf16_twin(dx.view(B, N, Dp), dxb), None, d_n1w, d_n1b, d_qkvw, d_qkvb, d_projw, d_projb, d_n2w, d_n2b, d_fc1w,
                 d_fc1b, d_fc2w, d_fc2b)
@@ -719,7 +719,7 @@ class Block(nn.Module):
     def forward_padded(self, xp: torch.Tensor) -> torch.Tensor:
         """xp fp32 [B,N,Dp] contiguous with zero pads -> same layout."""
         a, m = self.attn, self.mlp
-        fn = _BlockFn if self.saved_bits == 16 and isinstance(self.norm1, nn.LayerNorm) else _BlockActFn
+        fn = _BlockFn if self.saved_bits == 16 and norm_kind(self.norm1) == norm_kind(self.norm2) == "layer" else _BlockActFn
         return fn.apply(xp, self, self.norm1.weight, _norm_bias(self.norm1), a.qkv.weight, a.qkv.bias, a.proj.weight,
                         a.proj.bias, self.norm2.weight, _norm_bias(self.norm2), m.fc1.weight, m.fc1.bias, m.fc2.weight,
                         m.fc2.bias)
