@@ -30,3 +30,13 @@ def test_both_norms_choose_the_function_of_a_block(V, monkeypatch, first, second
     b.norm1, b.norm2 = first(16), second(16)
     b.forward_padded(torch.zeros(1, 2, 64))
     assert seen == [want]
+
+
+@pytest.mark.parametrize("norm,bits,want", [(nn.LayerNorm, 16, "_LayerNormFn"), (PlainNorm, 16, "_LayerNormFn"), (nn.RMSNorm, 16, "_NormActFn"),
+                                            (nn.LayerNorm, 8, "_NormActFn"), (PlainNorm, 8, "_NormActFn")])
+def test_a_norm_that_ran_before_runs_on_the_same_kernels(V, monkeypatch, norm, bits, want):
+    seen = []
+    for name in ("_LayerNormFn", "_NormActFn"):
+        monkeypatch.setattr(getattr(V, name), "apply", lambda *a, name=name: seen.append(name))
+    V.layer_norm_padded(torch.zeros(1, 2, 64), norm(16), bits)
+    assert seen == [want]

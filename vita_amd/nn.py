@@ -794,7 +794,7 @@ class _NormActFn(torch.autograd.Function):
 
 def layer_norm_padded(xp, ln, saved_bits=16):
     """nn.LayerNorm or nn.RMSNorm on the padded fp32 stream [B, N, Dp]."""
-    if saved_bits == 16 and isinstance(ln, nn.LayerNorm):
+    if saved_bits == 16 and norm_kind(ln) == "layer":
         return _LayerNormFn.apply(xp, ln.weight, ln.bias, ln.eps, ln.normalized_shape[0], ln)
     return _NormActFn.apply(xp, ln.weight, _norm_bias(ln), ln, saved_bits)
 
