@@ -79,3 +79,29 @@ def test_block_whose_norms_differ(V, first, second, bits):
     assert rel(x.grad, xr.grad) < tol
     for n, p in blk.named_parameters():
         assert rel(p.grad, P[n].grad) < tol, n
+
+
+# ------------------------------------------------------------------------------------------------ matrices that end with their last element
+@pytest.mark.parametrize("k,m,n", [(1, 1, 1), (1, 13, 40), (2, 15, 33), (64, 41, 64), (65, 6, 100), (130, 129, 257), (777, 300, 129), (129, 263, 4100),
+                                   (2000, 3075, 1025), (65, 4355, 4160), (300, 4403, 4000), (9001, 43, 40), (46082, 20, 20), (69262, 13, 6625)])
+def test_wgrad_of_a_dy_that_ends_with_its_last_element(V, k, m, n):
+    """dy's memory stops behind column m of the last token, inside a 16-byte piece; what would follow holds NaN in one of two runs and
+    does not exist for the caller in the other.  The last token counts in full, wherever its sum ends up (a tile, a part, a piece), and
+    a buffer's old values are added once."""
+    from vita_amd import ops
+    ld = -(-m // 8) * 8
+    g = torch.Generator(device="cuda").manual_seed(k + m + n)
+    x = torch.randn(k, -(-n // 8) * 8, device="cuda", generator=g).to(BF16)[:, :n]
+    x[-1] *= 8.0                                          # the last token weighs what the others do together
+    flat = torch.full(((k - 1) * ld + m,), float("nan"), dtype=BF16, device="cuda")
+    dy = flat.as_strided((k, m), (ld, 1))
+    dy.copy_(torch.randn(k, m, device="cuda", generator=g))
+    more = torch.cat([flat, torch.full((64,), float("nan"), dtype=BF16, device="cuda")])
+    a = ops.act8_pack(x)
+    dw = ops.act8_wgrad(dy, a)
+    v, d = ops.act8_unpack(a)[:, :n].double(), dy.double().t().contiguous()
+    tol = (8 * k ** 0.5 + 8) * U * (d.abs() @ v.abs()) + 1e-30       # k additions of exact products, as for every other weight gradient
+    assert ((dw.double() - d @ v).abs() <= tol).all()
+    assert torch.equal(dw, ops.act8_wgrad(more.as_strided((k, m), (ld, 1)), a))
+    start = torch.randn(m, n, device="cuda", generator=g)
+    assert torch.equal(ops.act8_wgrad(dy, a, out=start.clone()), start + dw)

@@ -144,6 +144,9 @@ __global__ __launch_bounds__(G2_THREADS, 2) void act8_wgrad_kernel(const Wgrad8P
 
     LoaderA la;
     la.init(P.dy + k0 * P.lddy, m0, P.m, krows, P.lddy, wave, lane);
+    // 16-byte pieces: the last one of the last token may reach behind the matrix' last element.  It is left out then (arrives as zeros)
+    // and its up to 7 columns of dy are added after the products.
+    if ((P.m & 7) && kt0 + nkt == P.kt) la.bytes -= 16;
     // bounds-checked loads: tokens past the part and columns past the codes arrive as zeros
     const uint32_t col_on = bcol < NF && n0 + bcol * 16 < ncodes;
     uint32_t qoff[2], soff[2];
@@ -286,6 +289,23 @@ __global__ __launch_bounds__(G2_THREADS, 2) void act8_wgrad_kernel(const Wgrad8P
 
     // lane: row lane & 15, columns 4 (lane >> 4) .. + 3 of each 16 x 16 fragment
     const int cl = wn * NFW * 16 + 4 * (lane >> 4), rl = wm * 64 + (lane & 15);
+    if ((P.m & 7) && kt0 + nkt == P.kt && P.m <= m0 + BM) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t row = m0 + rl + 16 * i;
+        if (row < (P.m & ~(int64_t)7) || row >= P.m) continue;
+        const float v = bf16_bits_to_f32(P.dy[(P.k - 1) * P.lddy + row]);
+#pragma unroll
+        for (int j = 0; j < NFW; ++j) {
+          const int64_t col = n0 + cl + 16 * j;
+          if (j >= nfw || col >= P.n) continue;
+          const int w = *reinterpret_cast<const int*>(P.q + (P.k - 1) * P.ldq + col);
+          const float s = v * act8_scale(P.scale[(P.k - 1) * P.lds + (col >> 5)]);       // an exact product, a power of two
+          acc[i][j] += f32x4{__builtin_amdgcn_cvt_f32_fp8(w, 0) * s, __builtin_amdgcn_cvt_f32_fp8(w, 1) * s, __builtin_amdgcn_cvt_f32_fp8(w, 2) * s,
+                             __builtin_amdgcn_cvt_f32_fp8(w, 3) * s};
+        }
+      }
+    }
     if (slot < 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
