@@ -40,3 +40,11 @@ def test_a_norm_that_ran_before_runs_on_the_same_kernels(V, monkeypatch, norm, b
         monkeypatch.setattr(getattr(V, name), "apply", lambda *a, name=name: seen.append(name))
     V.layer_norm_padded(torch.zeros(1, 2, 64), norm(16), bits)
     assert seen == [want]
+
+
+def test_a_linear_layer_that_keeps_8_bits_refuses_second_derivatives(V):
+    """Its backward pass is kernels: with create_graph=True its part would be missing.  Refused before any of them runs."""
+    from types import SimpleNamespace
+    ctx = SimpleNamespace(bits=8, saved_tensors=(None, None, None), dims=(1, 1, 64, 64, 16, 16), needs_input_grad=(True,) * 6)
+    with torch.enable_grad(), pytest.raises(RuntimeError, match="second derivatives"):
+        V._LinearFn.backward(ctx, torch.zeros(1, 1, 64))

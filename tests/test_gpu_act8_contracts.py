@@ -105,3 +105,14 @@ def test_wgrad_of_a_dy_that_ends_with_its_last_element(V, k, m, n):
     assert torch.equal(dw, ops.act8_wgrad(more.as_strided((k, m), (ld, 1)), a))
     start = torch.randn(m, n, device="cuda", generator=g)
     assert torch.equal(ops.act8_wgrad(dy, a, out=start.clone()), start + dw)
+
+
+# ------------------------------------------------------------------------------------------------ second derivatives
+def test_second_derivatives_of_an_8_bit_linear_layer_are_refused(V):
+    lin = nn.Linear(64, 32).cuda()
+    x = torch.randn(1, 5, 64, device="cuda", requires_grad=True)
+    f = lambda: V.linear_padded(x, lin, V._Shadows(), 64, 8)[..., :32].square().sum()
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(f(), x, create_graph=True)
+    want = 2 * torch.nn.functional.linear(x, lin.weight, lin.bias) @ lin.weight
+    assert rel(torch.autograd.grad(f(), x)[0], want) < BF16_TOL

@@ -550,12 +550,16 @@ def norm_bwd_padded(dy, src, rstd, ln, D, Dp, need_w, need_b, mean=None, dx_in=N
     return dx, dxb, dw, db
 
 
-def _first_order(backward):
+def _refuse_second_order():
     """For backward passes that are kernels: refuses create_graph=True, where their part would be missing from the second derivative."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("vita_amd: these kernels have no second derivatives (create_graph=True)")
+
+
+def _first_order(backward):
     @functools.wraps(backward)
     def run(ctx, *grads):
-        if torch.is_grad_enabled():
-            raise RuntimeError("vita_amd: these kernels have no second derivatives (create_graph=True)")
+        _refuse_second_order()
         return backward(ctx, *grads)
     return run
 
@@ -903,6 +907,8 @@ class _LinearFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        if ctx.bits == 8:
+            _refuse_second_order()
         *xs, ws = ctx.saved_tensors
         B, N, Kp, Np, out_f, in_f = ctx.dims
         M = B * N
