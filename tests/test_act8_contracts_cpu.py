@@ -48,3 +48,23 @@ def test_a_linear_layer_that_keeps_8_bits_refuses_second_derivatives(V):
     ctx = SimpleNamespace(bits=8, saved_tensors=(None, None, None), dims=(1, 1, 64, 64, 16, 16), needs_input_grad=(True,) * 6)
     with torch.enable_grad(), pytest.raises(RuntimeError, match="second derivatives"):
         V._LinearFn.backward(ctx, torch.zeros(1, 1, 64))
+
+
+def test_no_probe_for_a_second_stream_under_capture(V, monkeypatch):
+    """The probe waits for an event on the host, which ends a capture; a capture uses one stream anyway.  The next eager forward pass
+    probes then, and a stream that was found before is returned under capture too."""
+    dev = torch.device("cuda", 0)
+    monkeypatch.setattr(V, "_SIDE_STREAMS", {})
+    probes, capturing = [], [True]
+    monkeypatch.setattr(V, "_concurrent_stream", lambda idx, main: probes.append(idx) or "stream")
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda idx=None: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    assert V.ensure_side_stream(dev) is None and probes == [] and V._SIDE_STREAMS == {}
+    h = V._Shadows()
+    h._build["w"] = (lambda: None, None)
+    V.prefetch_shadows(dev)                             # nothing to fork to: the copies are rebuilt where they are used
+    assert probes == []
+    capturing[0] = False
+    assert V.ensure_side_stream(dev) == "stream" and probes == [0]
+    capturing[0] = True
+    assert V.ensure_side_stream(dev) == "stream" and probes == [0]

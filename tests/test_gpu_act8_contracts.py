@@ -116,3 +116,32 @@ def test_second_derivatives_of_an_8_bit_linear_layer_are_refused(V):
         torch.autograd.grad(f(), x, create_graph=True)
     want = 2 * torch.nn.functional.linear(x, lin.weight, lin.bias) @ lin.weight
     assert rel(torch.autograd.grad(f(), x)[0], want) < BF16_TOL
+
+
+# ------------------------------------------------------------------------------------------------ capture
+@pytest.mark.parametrize("bits", [8, 16])
+def test_the_first_block_of_a_device_inside_a_capture(V, monkeypatch, bits):
+    """No eager pass has chosen the second stream yet: the capture neither probes for it nor uses it, its replays equal eager passes
+    (weight gradients add at most 64 partial sums with atomics in any order: 64 half steps, and a factor 4), and the first eager pass
+    behind it probes."""
+    torch.manual_seed(2)
+    blk = V.Block(129, 3, 4.0, qkv_bias=True, saved_bits=bits).cuda()
+    x = torch.randn(2, 70, 129, device="cuda", requires_grad=True)
+    dy = torch.randn(2, 70, 129, device="cuda")
+    leaves = [x] + list(blk.parameters())
+    f = lambda: torch.autograd.grad(blk(x), leaves, dy)
+    f()                                                  # every library and copy that a capture may not create exists
+    torch.cuda.synchronize()
+    monkeypatch.setattr(V, "_SIDE_STREAMS", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = f()
+    assert V._SIDE_STREAMS == {}
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(2, 70, 129, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, f()):
+            assert rel(a, b) < 2.0 ** -16, k
+    assert len(V._SIDE_STREAMS) == 1

@@ -104,6 +104,8 @@ def prefetch_shadows(device):
     idx = device.index if device.index is not None else torch.cuda.current_device()
     main = torch.cuda.current_stream(idx)
     side = ensure_side_stream(device)
+    if side is None:
+        return                      # a capture before any eager pass
     side.wait_stream(main)          # after the optimizer step - and after every earlier use of the copies being replaced
     with torch.cuda.stream(side):
         for h in holders:
@@ -307,10 +309,13 @@ def ensure_side_stream(device, probe=True):
     on autograd's device thread after the reconstruction head's hooks could already have launched the first gradient
     bucket: gpurun_out/r2_share2.log shows one rank blocked there (e1.synchronize) while its peer waited for it inside
     the collective.  With probe=False (what a backward falls back to if no forward has run on this device) a plain
-    pool stream is taken without any host wait."""
+    pool stream is taken without any host wait.  A host wait would also end a capture, which uses one stream only: None then,
+    unless the stream is there already, and the next eager forward probes."""
     idx = device.index if getattr(device, "index", None) is not None else torch.cuda.current_device()
     s = _SIDE_STREAMS.get(idx)
     if s is None:
+        if probe and torch.cuda.is_current_stream_capturing():
+            return None
         s = _concurrent_stream(idx, torch.cuda.current_stream(idx)) if probe else torch.cuda.Stream(device=idx)
         _SIDE_STREAMS[idx] = s
     return s
