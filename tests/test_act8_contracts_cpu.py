@@ -68,3 +68,18 @@ def test_no_probe_for_a_second_stream_under_capture(V, monkeypatch):
     assert V.ensure_side_stream(dev) == "stream" and probes == [0]
     capturing[0] = True
     assert V.ensure_side_stream(dev) == "stream" and probes == [0]
+
+
+@pytest.mark.parametrize("capturing,enabled", [(True, True), (False, False)])
+def test_a_failed_backward_pass_does_not_swallow_later_reports(V, monkeypatch, capturing, enabled):
+    """An eager Block backward that raised leaves its list of deferred reports behind.  A later one on one stream (as under capture) has no
+    join that would hand it on: its accumulated gradients are reported at once."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    monkeypatch.setattr(V, "_DEFERRED_DONE", [])
+    p, seen = nn.Parameter(torch.zeros(1)), []
+    monkeypatch.setattr(V, "GRAD_READY", {id(p): seen.append})
+    side = V._SideStream(torch.device("cuda", 0), enabled)
+    assert not side.on
+    side(V.grad_done, p)
+    side.join()
+    assert len(seen) == 1 and seen[0] is p and V._DEFERRED_DONE is None

@@ -337,9 +337,10 @@ class _SideStream:
         # under capture everything stays on the capturing stream: a captured graph of two streams with several forks from one node has
         # been replayed with kernels before the ones they wait for (seen with plain element-wise kernels too)
         self.on = bool(enabled and WGRAD_SIDE_STREAM and not torch.cuda.is_current_stream_capturing())
-        if not self.on:
-            return
         global _DEFERRED_DONE
+        if not self.on:
+            _DEFERRED_DONE = None          # see below; here nothing would hand the reports on
+            return
         idx = device.index if device.index is not None else torch.cuda.current_device()
         self.main = torch.cuda.current_stream(idx)
         self.side = ensure_side_stream(device, probe=False)       # already chosen by the forward; never probes here
