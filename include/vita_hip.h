@@ -266,7 +266,7 @@ typedef struct vita_addnorm_fwd_desc {
   void* y;              /* optional [rows][ldy], y_dtype */
   void* q;              /* optional 8-bit rows of n (VITA_PACK_NORMED) or y (VITA_PACK_OUTPUT) */
   void* scale;
-  float* mean;          /* optional fp32 [rows] */
+  float* mean;          /* optional fp32 [rows]; written for VITA_NORM_LAYER only */
   float* rstd;          /* optional fp32 [rows] */
   int64_t rows, d;
   int64_t ldx, ldr, ldsum, ldy, ldq, lds;
@@ -284,7 +284,7 @@ typedef struct vita_addnorm_bwd_desc {
   const void* src;      /* s [rows][ldx], src_dtype, or NULL */
   const void* q;        /* 8-bit n, or NULL: exactly one of src and q */
   const void* scale;
-  const float* mean;    /* fp32 [rows]; needed for VITA_NORM_LAYER from src */
+  const float* mean;    /* fp32 [rows]; needed for VITA_NORM_LAYER from src, read for nothing else */
   const float* rstd;    /* fp32 [rows] */
   const float* gamma;   /* fp32 [d], or NULL = 1 */
   const void* dx_in;    /* optional gradient that reached s by other ways, [rows][lddx_in], dx_dtype */

@@ -145,3 +145,35 @@ def test_the_first_block_of_a_device_inside_a_capture(V, monkeypatch, bits):
         for a, b in zip(out, f()):
             assert rel(a, b) < 2.0 ** -16, k
     assert len(V._SIDE_STREAMS) == 1
+
+
+# ------------------------------------------------------------------------------------------------ the C entries' buffers
+def fwd_desc(ops, x, y, rstd, **kw):
+    from vita_amd import _lib
+    d = dict(x=x.data_ptr(), y=y.data_ptr(), rstd=rstd.data_ptr(), rows=x.shape[0], d=x.shape[1], ldx=x.stride(0), ldy=y.stride(0),
+             x_dtype=ops._dt(x), y_dtype=ops._dt(y), eps=1e-5)
+    return _lib.AddNormFwdDesc(**{**d, **kw})
+
+
+def bwd_desc(ops, dy, src, rstd, dx, **kw):
+    from vita_amd import _lib
+    d = dict(dy=dy.data_ptr(), src=src.data_ptr(), rstd=rstd.data_ptr(), dx=dx.data_ptr(), rows=dy.shape[0], d=dy.shape[1], lddy=dy.stride(0),
+             ldx=src.stride(0), lddx=dx.stride(0), dy_dtype=ops._dt(dy), src_dtype=ops._dt(src), dx_dtype=ops._dt(dx))
+    return _lib.AddNormBwdDesc(**{**d, **kw})
+
+
+def test_an_rms_norm_has_no_mean(V):
+    """A caller with one set of buffers for both kinds passes its mean along: the RMS norm neither writes nor reads it."""
+    import ctypes as C
+    from vita_amd import _lib, ops
+    rows, d = 40, 200
+    x, dy = torch.randn(rows, d, device="cuda"), torch.randn(rows, d, device="cuda")
+    y, dx, rstd = torch.empty_like(x), torch.empty_like(x), torch.empty(rows, device="cuda")
+    mean = torch.full((rows,), 7.0, device="cuda")
+    want = ops.addnorm_fwd(x, kind="rms", eps=1e-5, y_dtype=F32)
+    dwant, _, _ = ops.addnorm_bwd(dy, x, want.rstd, kind="rms", want_dgamma=False)
+    L = _lib.lib()
+    assert L.vita_addnorm_fwd(C.byref(fwd_desc(ops, x, y, rstd, mean=mean.data_ptr())), ops._s()) == 0
+    assert torch.equal(y, want.y) and torch.equal(rstd, want.rstd) and (mean == 7.0).all()
+    assert L.vita_addnorm_bwd(C.byref(bwd_desc(ops, dy, x, rstd, dx, mean=mean.data_ptr())), ops._s()) == 0
+    assert torch.equal(dx, dwant)

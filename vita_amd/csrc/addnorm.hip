@@ -463,7 +463,10 @@ extern "C" int vita_addnorm_bwd(const vita_addnorm_bwd_desc* dp, void* stream) {
   if (D.dx_in) VITA_REQUIRE(act8_mat_ok(D.dx_in, D.lddx_in, D.d, D.dx_dtype));
   if (D.dx_bf16) VITA_REQUIRE(act8_mat_ok(D.dx_bf16, D.lddxb, D.d, VITA_DT_BF16));
   VITA_REQUIRE((D.partial != nullptr) == (D.dgamma || D.dbeta));
-  if (D.kind == AN_RMS) VITA_REQUIRE(!D.dbeta);
+  if (D.kind == AN_RMS) {
+    VITA_REQUIRE(!D.dbeta);
+    D.mean = nullptr;                   // mu = 0
+  }
   int64_t width = (D.d + 7) & ~(int64_t)7;
   if (D.lddx > width) width = D.lddx;
   if (D.dx_bf16 && D.lddxb > width) width = D.lddxb;
