@@ -177,3 +177,50 @@ def test_an_rms_norm_has_no_mean(V):
     assert torch.equal(y, want.y) and torch.equal(rstd, want.rstd) and (mean == 7.0).all()
     assert L.vita_addnorm_bwd(C.byref(bwd_desc(ops, dy, x, rstd, dx, mean=mean.data_ptr())), ops._s()) == 0
     assert torch.equal(dx, dwant)
+
+
+def wide(rows, d, dtype, seed, ld):
+    """[rows, d] on rows of ld elements, NaN behind each; ends with its last element."""
+    t = torch.full((rows, ld), float("nan"), dtype=dtype, device="cuda")
+    t[:, :d] = torch.randn(rows, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).to(dtype)
+    return t[:, :d]
+
+
+@pytest.mark.parametrize("rows,d", [(1, 5), (41, 69), (70, 130), (70, 300), (2100, 777), (40, 777), (2100, 1025), (70, 1025), (1500, 1500), (40, 1601),
+                                    (40, 2636), (40, 5001), (40, 7003)])
+def test_outputs_in_place_of_inputs(V, rows, d):
+    """The sum in place of x or of the residual, dx in place of dx_in, dz in place of dg: the same bits as in memory of their own, with
+    rows that leave no room between them (4 fp32 columns behind a row are the next row's)."""
+    import ctypes as C
+    from vita_amd import _lib, ops
+    L = _lib.lib()
+    gamma = (1 + 0.2 * torch.randn(d, device="cuda")).contiguous()
+    for dtype, step in ((F32, 4), (BF16, 8)):
+        ld = -(-d // step) * step
+        x, res = wide(rows, d, dtype, 1, ld), wide(rows, d, dtype, 2, ld)
+        want = ops.addnorm_fwd(x, gamma, residual=res, eps=1e-5, y_dtype=BF16, sum_dtype=dtype, pack="normed")
+        for place in ("x", "res"):
+            t = {k: wide(rows, d, dtype, 0, ld).copy_(v) for k, v in (("x", x), ("res", res))}
+            y, rstd = torch.empty_like(want.y), torch.empty_like(want.rstd)
+            q, s = torch.empty_like(want.act.q), torch.empty_like(want.act.scale)
+            desc = fwd_desc(ops, t["x"], y, rstd, gamma=gamma.data_ptr(), res=t["res"].data_ptr(), ldr=ld, res_dtype=ops._dt(res),
+                            sum=t[place].data_ptr(), ldsum=ld, sum_dtype=ops._dt(x), q=q.data_ptr(), scale=s.data_ptr(), ldq=q.stride(0),
+                            lds=s.shape[1])
+            desc.d, desc.ldx, desc.ldy = d, ld, y.stride(0)
+            assert L.vita_addnorm_fwd(C.byref(desc), ops._s()) == 0
+            assert torch.equal(t[place], want.sum[:, :d]) and torch.equal(y, want.y) and torch.equal(rstd, want.rstd)
+            assert torch.equal(q.view(torch.uint8), want.act.q.view(torch.uint8)) and torch.equal(s.view(torch.uint8), want.act.scale.view(torch.uint8))
+        src, dy, dx_in = wide(rows, d, dtype, 3, ld), wide(rows, d, dtype, 4, ld), wide(rows, d, dtype, 5, ld)
+        dwant, _, _ = ops.addnorm_bwd(dy, src, want.rstd, gamma, dx_in=dx_in, dx_dtype=dtype, want_dgamma=False)
+        desc = bwd_desc(ops, dy, src, want.rstd, dx_in, gamma=gamma.data_ptr(), dx_in=dx_in.data_ptr(), lddx_in=ld)
+        desc.lddy = desc.ldx = desc.lddx = ld
+        assert L.vita_addnorm_bwd(C.byref(desc), ops._s()) == 0
+        assert torch.equal(dx_in, dwant[:, :d])
+    ld = -(-d // 8) * 8
+    dg = wide(rows, d, BF16, 6, ld)
+    _, act = ops.gelu_act8_fwd(wide(rows, d, BF16, 7, ld))
+    want, g = ops.gelu_act8_bwd(dg, act)
+    g2 = torch.empty_like(g)
+    assert L.vita_gelu_act8_bwd(dg.data_ptr(), ld, act.q.data_ptr(), act.q.stride(0), act.scale.data_ptr(), act.scale.shape[1], rows, d,
+                                dg.data_ptr(), ld, g2.data_ptr(), ld, ops._s()) == 0
+    assert torch.equal(dg, want[:, :d]) and torch.equal(g2, g)
