@@ -253,8 +253,10 @@ int vita_act8_wgrad(const void* dy, int64_t lddy, const void* q, int64_t ldq, co
 
 /* ------------------------------------------------------------------ residual addition + norm, with an 8-bit output
  * s = x + res;  n = (s - mu) * rstd, rstd = 1 / sqrt(mean((s - mu)^2) + eps), mu = 0 (VITA_NORM_RMS: nn.RMSNorm) or mean(s)
- * (VITA_NORM_LAYER: nn.LayerNorm, networks/imaging_encoders.py:41,115);  y = n * gamma (+ beta).  All in fp32; s, y and the 8-bit
- * rows are each rounded once from it (n does not see the rounding of s).  Rows of up to 8192 columns, pads included. */
+ * (VITA_NORM_LAYER: nn.LayerNorm, networks/imaging_encoders.py:41,115);  y = n * gamma (+ beta).  In fp32, summed in 64 bits;
+ * s, y and the 8-bit rows are each rounded once from it (n does not see the rounding of s to its type), and next to a border between
+ * two codes n and y are taken in 64 bits: the codes are those of the exact norm of the fp32 s (but for values that beta cancels to a
+ * sixteenth and less).  Rows of up to 8192 columns, pads included. */
 enum { VITA_NORM_RMS = 0, VITA_NORM_LAYER = 1 };
 enum { VITA_PACK_NORMED = 0, VITA_PACK_OUTPUT = 1 };
 typedef struct vita_addnorm_fwd_desc {

@@ -224,3 +224,31 @@ def test_outputs_in_place_of_inputs(V, rows, d):
     assert L.vita_gelu_act8_bwd(dg.data_ptr(), ld, act.q.data_ptr(), act.q.stride(0), act.scale.data_ptr(), act.scale.shape[1], rows, d,
                                 dg.data_ptr(), ld, g2.data_ptr(), ld, ops._s()) == 0
     assert torch.equal(dg, want[:, :d]) and torch.equal(g2, g)
+
+
+# ------------------------------------------------------------------------------------------------ which of two codes
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("pack", ["normed", "output"])
+@pytest.mark.parametrize("rows,d", [(60000, 29), (30000, 100), (15000, 200), (9000, 300), (5000, 600), (4000, 1025), (700, 1025), (4000, 1060),
+                                    (3000, 1500), (2000, 2000), (1000, 4000), (600, 7000)])
+def test_codes_are_those_of_the_64_bit_norm(V, rows, d, kind, pack):
+    """x and the residual are multiples of 2^-8 below 8, so that their sum is exact in 32 bits; no beta, whose addition may cancel.  What
+    is left of the norm's own arithmetic then is a few 2^-52: the codes and the scales are those of the 64-bit formula, value by value,
+    where 32 bits would put about one in two million on the other side of a border (a step of 2^-3)."""
+    from vita_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(rows + d)
+    mk = lambda: ((torch.randn(rows, -(-d // 8) * 8, device="cuda", generator=g) * 128).round().clamp(-1024, 1024) / 256).to(BF16)[:, :d]
+    x, res = mk(), mk()
+    gamma = 1 + 0.2 * torch.randn(d, device="cuda", generator=g)
+    wrong = total = 0
+    for r in (None, res):
+        a = ops.addnorm_fwd(x, gamma, residual=r, kind=kind, eps=1e-5, y_dtype=None, pack=pack)
+        s = x.double() if r is None else x.double() + r.double()
+        assert torch.equal(s.float().double(), s)
+        n = s - s.mean(1, keepdim=True) if kind == "layer" else s
+        n = n / torch.sqrt(n.square().mean(1, keepdim=True) + 1e-5)
+        # on the CPU: powers of two from the device's pow are not all exact
+        want, scale = R.quantise((n * gamma.double() if pack == "output" else n).cpu())
+        wrong += (R.values(a.act) != want).sum().item() + (a.act.scale.view(torch.uint8).cpu() != scale).sum().item()
+        total += want.numel()
+    assert wrong == 0, (wrong, total)

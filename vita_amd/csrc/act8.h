@@ -37,13 +37,12 @@ __device__ __forceinline__ float act8_inv_scale(uint32_t byte) { return __builti
 // at its end and values saturate
 #define ACT8_TOP 0x7f600000u
 
-// the 8 values of a lane (all 4 lanes of the quad call it) -> their codes; byte = the group's scale byte
-__device__ __forceinline__ u32x2 act8_encode(const float (&v)[8], uint32_t& byte) {
-  uint32_t m = 0;
+// the 8 values of a lane (all 4 lanes of the quad call it) over their group's scale: t, the scale byte and the bits of the largest magnitude
+__device__ __forceinline__ void act8_scaled(const float (&v)[8], float (&t)[8], uint32_t& byte, uint32_t& m) {
+  m = 0;
 #pragma unroll
   for (int r = 0; r < 8; ++r) { const uint32_t a = __builtin_bit_cast(uint32_t, v[r]) & 0x7fffffffu; m = m > a ? m : a; }
   m = act8_quad_max(m);
-  float t[8];
   if (__builtin_expect(m > ACT8_TOP, 0)) {      // the four lanes of a quad together
     m = 0;
 #pragma unroll
@@ -51,7 +50,8 @@ __device__ __forceinline__ u32x2 act8_encode(const float (&v)[8], uint32_t& byte
       const uint32_t a = __builtin_bit_cast(uint32_t, v[r]) & 0x7fffffffu;
       if (a < 0x7f800000u) m = m > a ? m : a;
     }
-    byte = act8_scale_byte(act8_quad_max(m));
+    m = act8_quad_max(m);
+    byte = act8_scale_byte(m);
     const float inv = act8_inv_scale(byte);
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
@@ -64,6 +64,8 @@ __device__ __forceinline__ u32x2 act8_encode(const float (&v)[8], uint32_t& byte
 #pragma unroll
     for (int r = 0; r < 8; ++r) t[r] = v[r] * inv;
   }
+}
+__device__ __forceinline__ u32x2 act8_codes(const float (&t)[8]) {
   u32x2 q;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -73,6 +75,17 @@ __device__ __forceinline__ u32x2 act8_encode(const float (&v)[8], uint32_t& byte
   }
   return q;
 }
+// the 8 values of a lane (all 4 lanes of the quad call it) -> their codes; byte = the group's scale byte
+__device__ __forceinline__ u32x2 act8_encode(const float (&v)[8], uint32_t& byte) {
+  float t[8];
+  uint32_t m;
+  act8_scaled(v, t, byte, m);
+  return act8_codes(t);
+}
+// Whether a value over its scale lies within w steps of 2^-23 of a border between two codes (normal ones: 3 bits of the mantissa, a border
+// half a step behind each), or a group's maximum within w of the border between two scales (1.75 2^k)
+__device__ __forceinline__ uint32_t act8_off_border(float t, uint32_t w) { return (__builtin_bit_cast(uint32_t, t) + 0x80000u + w) & 0xfffffu; }     // <= 2 w
+__device__ __forceinline__ bool act8_near_scale(uint32_t m, uint32_t w) { return (m & 0x7fffffu) - 0x600000u + w <= 2 * w; }
 __device__ __forceinline__ void act8_decode(u32x2 q, uint32_t byte, float (&v)[8]) {
   typedef float f32x2v __attribute__((ext_vector_type(2)));
   const float s = act8_scale(byte);

@@ -2,16 +2,17 @@
 // from the 8-bit rows or from the kept sum.
 //
 //   s = x + r                                  (fp32; written rounded to its type when asked for)
-//   mu = 0 (rms) | mean(s) (layer);  rstd = 1 / sqrt(mean((s - mu)^2) + eps)       two passes over registers, fp32
+//   mu = 0 (rms) | mean(s) (layer);  rstd = 1 / sqrt(mean((s - mu)^2) + eps)       two passes over registers, summed in 64 bits
 //   n = (s - mu) rstd;  y = n gamma [+ beta]   y in bf16 / fp32, and n or y in 8 bits (act8.h)
 // backward, with h = dy gamma:
 //   dx = dx_in + rstd (h - [mean(h)] - n mean(h n)),  dgamma = sum_rows dy n,  dbeta = sum_rows dy
 // n comes from the 8-bit rows (1.03 bytes a value and rstd) or from s and (mu, rstd).
 //
 // Both move bytes.  Measured (MI355X, kernels alone; a copy of that size reaches 5 TB/s):
-//   forward, 46082 x 1025, bf16 + fp32 -> fp32 sum, bf16 y, 8-bit n: 133 us, 4.8 TB/s (one wave per row and a row per block of gamma
+//   forward, 46082 x 1025, bf16 + fp32 -> fp32 sum, bf16 y, 8-bit n: 130 us, 4.8 TB/s (one wave per row and a row per block of gamma
 //     and beta loads: 186 us; rows dealt to resident waves with gamma in registers: 141 us; 64 columns behind the chunks one to a
-//     lane: 134 us)
+//     lane: 134 us; all of it in 64 bits instead of the sums and the values next to a border: 134 us, with a LayerNorm's 8-bit output of bf16 +
+//     bf16 107 instead of 95)
 //   backward, 13826 x 1025, from 8 bits, bf16 dy, fp32 dx_in and dx: 37 + 4 us (sums of the partial rows), 4.5 TB/s (gamma read
 //     anew for each row and dx_in after the sums: 89 + 16 us; loads together, gamma in registers: 61; 768 partial rows of 1025
 //     columns added with all loads in flight: 4 instead of 16 us; last columns one to a lane, 3 blocks a CU instead of 2: 37; with
@@ -30,11 +31,44 @@
 #define AN_FULL 0
 #define AN_TAIL 1
 
-// sums over the W waves that share a row (W = 1: the wave itself, or its L neighbouring lanes, no barrier), two at a time
-template <int W, int L>
-__device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2][W], int& turn, int wave, int lane) {
+// A wave's sums of doubles in all of its lanes (or its L neighbouring ones) without LDS: quads, halves and whole rows of 16 lanes by DPP
+// (mirrored: the lanes that differ in lower bits hold the same sum by then), rows and halves of the wave by swaps
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xf, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, true);
+  return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int O>
+__device__ __forceinline__ double swap_add(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)b, hi = (uint32_t)(b >> 32);
+  const auto p = O == 16 ? __builtin_amdgcn_permlane16_swap(lo, lo, false, false) : __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+  const auto q = O == 16 ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false) : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+  return __builtin_bit_cast(double, (uint64_t)q[0] << 32 | p[0]) + __builtin_bit_cast(double, (uint64_t)q[1] << 32 | p[1]);
+}
+template <int L>
+__device__ __forceinline__ double lane_sum(double v) {
+  v = dpp_add<0xB1>(v);                 // quad_perm [1,0,3,2]
+  v = dpp_add<0x4E>(v);                 // quad_perm [2,3,0,1]
+  v = dpp_add<0x141>(v);                // row_half_mirror
+  v = dpp_add<0x140>(v);                // row_mirror
+  if (L > 16) v = swap_add<16>(v);
+  if (L > 32) v = swap_add<32>(v);
+  return v;
+}
+template <int L>
+__device__ __forceinline__ void lane_sum2(double& a, double& b) { a = lane_sum<L>(a); b = lane_sum<L>(b); }
+template <int L>
+__device__ __forceinline__ void lane_sum2(float& a, float& b) {
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
+}
+// sums over the W waves that share a row (W = 1: the wave itself, or its L neighbouring lanes, no barrier), two at a time
+template <int W, int L, typename F>
+__device__ __forceinline__ void row_sum2(F& a, F& b, F (*red)[2][W], int& turn, int wave, int lane) {
+  lane_sum2<L>(a, b);
   if (W == 1) return;
   turn ^= 1;                          // two slots in turn: the barrier of the next sum lies between a slot's reads and its next writes
   if (lane == 0) { red[turn][0][wave] = a; red[turn][1][wave] = b; }
@@ -44,9 +78,8 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2][W],
   for (int w = 1; w < W; ++w) { a += red[turn][0][w]; b += red[turn][1][w]; }
 }
 template <int W, int L>
-__device__ __forceinline__ float row_sum(float a, float (*red)[2][W], int& turn, int wave, int lane) {
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) a += __shfl_xor(a, o, 64);
+__device__ __forceinline__ double row_sum(double a, double (*red)[2][W], int& turn, int wave, int lane) {
+  a = lane_sum<L>(a);
   if (W == 1) return a;
   turn ^= 1;
   if (lane == 0) red[turn][0][wave] = a;
@@ -57,15 +90,24 @@ __device__ __forceinline__ float row_sum(float a, float (*red)[2][W], int& turn,
   return a;
 }
 
+// A double as the float next to it towards zero, its last bit set where that is not exact: on the same side of every number of fewer
+// bits (the borders between 8-bit codes, the maxima at which a scale changes) as the double itself
+__device__ __forceinline__ float odd_float(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t rest = (uint32_t)b & 0x1fffffffu;
+  const float f = (float)__builtin_bit_cast(double, b & ~(uint64_t)0x1fffffffu);
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, f) | (rest ? 1u : 0u));
+}
+
 // A wave (W = 1) or the four waves of a block (W = 4) walk over rows, 8 neighbouring columns to a lane and chunk, the row in
 // registers from its loads to its stores; gamma and beta stay in registers.  T: up to 64 columns behind the last whole chunk go one to
 // a lane instead of opening another chunk (1025 columns would fill 1 of its 64 lanes and cost every lane 8 columns of registers and
 // arithmetic).  M = 16, 32: narrow rows, 4 or 2 of them to a wave.
-template <int W, int NV, int M, bool XF, int RT>      // RT: 0 no residual, 1 bf16, 2 fp32
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void addnorm_fwd_kernel(const vita_addnorm_fwd_desc D, const int al) {
+template <int W, int NV, int M, bool XF, int RT, bool LAYER>      // RT: 0 no residual, 1 bf16, 2 fp32
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, NV == 2 ? 4 : 1) void addnorm_fwd_kernel(const vita_addnorm_fwd_desc D, const int al) {
   constexpr bool T = M == AN_TAIL;
   constexpr int L = M > AN_TAIL ? M : 64, R = W == 1 ? 256 / L : 1;      // lanes of a wave to a row; rows of a block at a time
-  __shared__ float red[2][2][W];
+  __shared__ double red[2][2][W];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int d = (int)D.d, t0 = (W == 1 ? lane % L : (int)threadIdx.x) * 8;
   const double inv_d = 1.0 / (double)d;
@@ -93,7 +135,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void addnorm_fwd_kernel(cons
       vt = load1<XF>((const char*)D.x + row * D.ldx * (XF ? 4 : 2), ct, d);
       if (RT) vt += load1<RT == 2>((const char*)D.res + row * D.ldr * (RT == 2 ? 4 : 2), ct, d);
     }
-    float v[NV][8], s = vt;
+    float v[NV][8];
+    const auto clear = [&](int i, float (&a)[8]) {       // behind the row's end
+      const int c = t0 + i * W * 512;
+      if (c + 8 > d) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) if (c + r >= d) a[r] = 0.f;
+      }
+    };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       raw_values8<XF>(xr[i], v[i]);
@@ -103,80 +152,104 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void addnorm_fwd_kernel(cons
 #pragma unroll
         for (int r = 0; r < 8; ++r) v[i][r] += t[r];
       }
-      if (t0 + i * W * 512 + 8 > d) {
-#pragma unroll
-        for (int r = 0; r < 8; ++r) if (t0 + i * W * 512 + r >= d) v[i][r] = 0.f;
-      }
-#pragma unroll
-      for (int r = 0; r < 8; ++r) s += v[i][r];
+      clear(i, v[i]);
     }
     if (RT && D.sum) {
+      const bool f = D.sum_dtype == VITA_DT_F32;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) store8((char*)D.sum + row * D.ldsum * (f ? 4 : 2), t0 + i * W * 512, D.ldsum, f, v[i]);
+      if (T) store1((char*)D.sum + row * D.ldsum * (f ? 4 : 2), ct, D.ldsum, f, vt);
+    }
+    const auto forget = [&]() {         // the 64-bit form of v, or it would be held from one use to the next: 16 NV registers
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        store8((char*)D.sum + row * D.ldsum * (D.sum_dtype == VITA_DT_F32 ? 4 : 2), t0 + i * W * 512, D.ldsum, D.sum_dtype == VITA_DT_F32, v[i]);
-      if (T) store1((char*)D.sum + row * D.ldsum * (D.sum_dtype == VITA_DT_F32 ? 4 : 2), ct, D.ldsum, D.sum_dtype == VITA_DT_F32, vt);
-    }
-    if (D.kind == AN_LAYER) {
-      const float mu = (float)(row_sum<W, L>(s, red, turn, wave, lane) * inv_d);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) asm volatile("" : "+v"(v[i][r]));
+    };
+    double mu = 0.0;
+    if (LAYER) {
+      double s = (double)vt;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int r = 0; r < 8; ++r) v[i][r] -= mu;
-      if (T && ct < d) vt -= mu;
-      if (D.mean && t0 == 0) D.mean[row] = mu;
+        for (int r = 0; r < 8; ++r) s += (double)v[i][r];
+      mu = row_sum<W, L>(s, red, turn, wave, lane) * inv_d;
+      if (D.mean && t0 == 0) D.mean[row] = (float)mu;
+      forget();
     }
-    float q = T ? vt * vt : 0.f;
+    double q = T && ct < d ? ((double)vt - mu) * ((double)vt - mu) : 0.0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = t0 + i * W * 512;
-      if (c + 8 > d) {
+      double a[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) if (c + r >= d) v[i][r] = 0.f;
+      for (int r = 0; r < 8; ++r) a[r] = LAYER ? (double)v[i][r] - mu : (double)v[i][r];
+      if (LAYER && c + 8 > d) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) if (c + r >= d) a[r] = 0.0;
       }
 #pragma unroll
-      for (int r = 0; r < 8; ++r) q = __builtin_fmaf(v[i][r], v[i][r], q);
+      for (int r = 0; r < 8; ++r) q = __builtin_fma(a[r], a[r], q);
     }
-    // rstd as a pair of floats from 64 bits, n rounded once from its product: an error in the last bit of rstd would send ten times as
-    // many values across the borders of the 8-bit codes as the roundings that are left
-    const double r = 1.0 / sqrt((double)row_sum<W, L>(q, red, turn, wave, lane) * inv_d + (double)D.eps);
-    const float rs = (float)r, rl = (float)(r - (double)rs);
-    if (D.rstd && t0 == 0) D.rstd[row] = rs;
+    forget();
+    const double rs = 1.0 / sqrt(row_sum<W, L>(q, red, turn, wave, lane) * inv_d + (double)D.eps);
+    // mu and rstd as pairs of floats: s - mu and n are each rounded as if from 64 bits, up to 3 steps of 2^-24 in all
+    const float rh = (float)rs, rl = (float)(rs - (double)rh), mh = (float)mu, ml = (float)(mu - (double)mh);
+    if (D.rstd && t0 == 0) D.rstd[row] = rh;
+    // A rounding that carries a value across a border between two codes changes the code by a whole step of 2^-3: where one comes within
+    // `near` steps of 2^-23 of a border, its chunk is computed once more in 64 bits (a wave in 120 normed ones, in 30 of outputs, whose
+    // beta may cancel some bits)
+    const bool out = D.pack == VITA_PACK_OUTPUT;
+    const uint32_t near = out ? 32 : 8;
     const int dq = (d + 31) & ~31;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = t0 + i * W * 512;
-      float y[8];
+      float n[8], y[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        v[i][r] = __builtin_fmaf(v[i][r], rs, v[i][r] * rl);
-        y[r] = __builtin_fmaf(v[i][r], gm[i][r], bt[i][r]);
+        const float a = LAYER ? (v[i][r] - mh) - ml : v[i][r];
+        n[r] = __builtin_fmaf(a, rh, a * rl);
+        y[r] = __builtin_fmaf(n[r], gm[i][r], bt[i][r]);
       }
-      if (c + 8 > d) {                         // zeros behind the row's end, also in a row whose rstd is NaN
-#pragma unroll
-        for (int r = 0; r < 8; ++r) if (c + r >= d) v[i][r] = y[r] = 0.f;
-      }
+      clear(i, n);                             // also in a row whose rstd is NaN
+      clear(i, y);
+      if (D.y) store8((char*)D.y + row * D.ldy * (D.y_dtype == VITA_DT_F32 ? 4 : 2), c, D.ldy, D.y_dtype == VITA_DT_F32, y);
       if (D.q) {
-        uint32_t byte;
-        const u32x2 w = D.pack == VITA_PACK_OUTPUT ? act8_encode(y, byte) : act8_encode(v[i], byte);
+        uint32_t byte, m, off = 0xffffffffu;
+        float t[8];
+        if (out) act8_scaled(y, t, byte, m); else act8_scaled(n, t, byte, m);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) { const uint32_t o = act8_off_border(t[r], near); off = off < o ? off : o; }
+        u32x2 w = act8_codes(t);
+        if (__builtin_expect(__any(off <= 2 * near || act8_near_scale(m, near)), 0)) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            float a = v[i][r], b = gm[i][r], e = bt[i][r];
+            asm volatile("" : "+v"(a), "+v"(b), "+v"(e));      // or their 64-bit forms would be held in registers from the row's start
+            const double u = ((double)a - mu) * rs;
+            t[r] = odd_float(out ? __builtin_fma(u, (double)b, (double)e) : u);
+          }
+          clear(i, t);
+          w = act8_encode(t, byte);
+        }
         if (c < dq) {
           *reinterpret_cast<u32x2*>((uint8_t*)D.q + row * D.ldq + c) = w;
           if ((c & 31) == 0) ((uint8_t*)D.scale)[row * D.lds + (c >> 5)] = (uint8_t)byte;
         }
       }
-      if (D.y) store8((char*)D.y + row * D.ldy * (D.y_dtype == VITA_DT_F32 ? 4 : 2), c, D.ldy, D.y_dtype == VITA_DT_F32, y);
     }
-    if (T) {
-      vt = ct < d ? __builtin_fmaf(vt, rs, vt * rl) : 0.f;
-      const float y = ct < d ? __builtin_fmaf(vt, gt, btt) : 0.f;
+    if (T) {                                   // one value: in 64 bits at once
+      const double n = ((double)vt - mu) * rs;
       if (D.q) {
         uint32_t byte;
-        const uint8_t w = act8_encode1(D.pack == VITA_PACK_OUTPUT ? y : vt, byte);
+        const uint8_t w = act8_encode1(ct < d ? odd_float(out ? __builtin_fma(n, (double)gt, (double)btt) : n) : 0.f, byte);
         if (ct < dq) {
           ((uint8_t*)D.q)[row * D.ldq + ct] = w;
           if ((ct & 31) == 0) ((uint8_t*)D.scale)[row * D.lds + (ct >> 5)] = (uint8_t)byte;
         }
       }
-      if (D.y) store1((char*)D.y + row * D.ldy * (D.y_dtype == VITA_DT_F32 ? 4 : 2), ct, D.ldy, D.y_dtype == VITA_DT_F32, y);
+      if (D.y) store1((char*)D.y + row * D.ldy * (D.y_dtype == VITA_DT_F32 ? 4 : 2), ct, D.ldy, D.y_dtype == VITA_DT_F32, ct < d ? __builtin_fmaf((float)n, gt, btt) : 0.f);
     }
   }
 }
@@ -210,8 +283,12 @@ extern "C" int vita_addnorm_fwd(const vita_addnorm_fwd_desc* dp, void* stream) {
     const int64_t at_once = w > 1 ? 1 : m > AN_TAIL ? 256 / m : 4, n = (D.rows + at_once - 1) / at_once;
     return n < AN_FWD_MAXBLK ? n : AN_FWD_MAXBLK;
   };
-#define AN_LAUNCH(W, NV, M, XF, RT) \
-  hipLaunchKernelGGL((addnorm_fwd_kernel<W, NV, M, XF, RT>), dim3((unsigned)(blocks(W, M))), dim3(W == 1 ? 256 : 64 * W), 0, (hipStream_t)stream, D, al)
+#define AN_LAUNCH(W, NV, M, XF, RT)                                                                                                          \
+  do {                                                                                                                                       \
+    const dim3 g((unsigned)blocks(W, M)), b(W == 1 ? 256 : 64 * W);                                                                          \
+    if (D.kind == AN_LAYER) hipLaunchKernelGGL((addnorm_fwd_kernel<W, NV, M, XF, RT, true>), g, b, 0, (hipStream_t)stream, D, al);           \
+    else hipLaunchKernelGGL((addnorm_fwd_kernel<W, NV, M, XF, RT, false>), g, b, 0, (hipStream_t)stream, D, al);                             \
+  } while (0)
 #define AN_TYPES(W, NV, M)                                                                                                                   \
   do {                                                                                                                                       \
     if (D.x_dtype == VITA_DT_F32) {                                                                                                          \
@@ -223,8 +300,9 @@ extern "C" int vita_addnorm_fwd(const vita_addnorm_fwd_desc* dp, void* stream) {
   // Few rows: four waves to a row shorten the way through one row, many rows: a wave to each saves the barriers.  One wave / four, us,
   // bf16 + fp32 residual, 600 columns: 1 row 3.7 / 3.0, 512 rows 5.3 / 4.8, 1024 5.8 / 6.0, 2048 7.0 / 8.7; 1025 columns: 3.8 / 3.2,
   // 5.6 / 5.2, 6.2 / 6.3, 8.3 / 9.7.  Above 1536 columns a wave would hold 4 chunks and more (64 registers of values): four waves, with
-  // one chunk a lane as far as that goes (2000 columns, 8192 rows: 34.0 us, with two chunks, half of them empty, 36.6; from 2049 to
-  // 8192 columns more waves with one chunk each gain nothing, 119 us against 139 at 9000 x 5000).  Narrow rows share a wave: 46082 rows
+  // one chunk a lane as far as that goes (2000 columns, 8192 rows: 34.0 us, with two chunks, half of them empty, 36.6).  Above 4096 columns
+  // eight waves with two chunks a lane, in whose registers four of them fit a SIMD (four waves with four chunks, two of which fit: 9000 x
+  // 5000, fp32, 153 against 140 us; 6000 x 4106 91 against 84; 16 x 4600 the same).  Narrow rows share a wave: 46082 rows
   // of 69 columns, 16 lanes each 11.2 us, 64 lanes 24.4; of 130 columns, 32 lanes 15.9 us, 64 lanes 24.6.
   if (width <= 128) AN_TYPES(1, 1, 16);
   else if (width <= 256) AN_TYPES(1, 1, 32);
@@ -234,7 +312,7 @@ extern "C" int vita_addnorm_fwd(const vita_addnorm_fwd_desc* dp, void* stream) {
   else if (width <= 1088) AN_TYPES(1, 2, AN_TAIL);
   else if (width <= 1536) AN_TYPES(1, 3, AN_FULL);
   else if (width <= 4096) AN_TYPES(4, 2, AN_FULL);
-  else AN_TYPES(4, 4, AN_FULL);
+  else AN_TYPES(8, 2, AN_FULL);
 #undef AN_TYPES
 #undef AN_LAUNCH
   VITA_CHECK_LAUNCH("vita_addnorm_fwd");
