@@ -305,10 +305,9 @@ def ensure_side_stream(device, probe=True):
 
     The probe blocks the host on an event, so it must run where nothing else can be waiting for this thread: from the
     constructors of FlatAdam / BucketedAllReduce and from the first Block FORWARD (main thread, no collective of the
-    step in flight yet) - never from a Block backward.  Round 2 probed lazily inside the first _BlockFn.backward, i.e.
-    on autograd's device thread after the reconstruction head's hooks could already have launched the first gradient
-    bucket: gpurun_out/r2_share2.log shows one rank blocked there (e1.synchronize) while its peer waited for it inside
-    the collective.  With probe=False (what a backward falls back to if no forward has run on this device) a plain
+    step in flight yet) - never from a Block backward: probed inside the first _BlockFn.backward, i.e. on autograd's
+    device thread after the reconstruction head's hooks could already have launched the first gradient bucket, one rank
+    was blocked there (e1.synchronize) while its peer waited for it inside the collective.  With probe=False (what a backward falls back to if no forward has run on this device) a plain
     pool stream is taken without any host wait.  A host wait would also end a capture, which uses one stream only: None then,
     unless the stream is there already, and the next eager forward probes."""
     idx = device.index if getattr(device, "index", None) is not None else torch.cuda.current_device()
@@ -575,8 +574,9 @@ class _BlockActFn(torch.autograd.Function):
     token then: the two norms' normalised rows (from which their own gradients AND the weight gradients of the products behind
     them are computed), the MLP's pre-activation (GELU and GELU' both follow from it), all in 8 bits, and q, k, v and the
     attention output in bf16: the backward pass recomputes the probabilities from q, k and the saved log-sum-exp, and 8-bit
-    scores would no longer sum to one against it.  About 14.5 bytes per token and channel instead of 36; the forward pass itself
-    computes with unrounded activations."""
+    scores would no longer sum to one against it.  About 15 bytes per token and channel instead of 33.5.  The forward pass itself
+    computes with the values as they are before they are stored; the MLP's pre-activation passes through bf16 on its way to GELU,
+    where the 16-bit Block takes GELU of the fp32 sums."""
 
     @staticmethod
     def forward(ctx, xp, blk, n1w, n1b, qkvw, qkvb, projw, projb, n2w, n2b, fc1w, fc1b, fc2w, fc2b):
